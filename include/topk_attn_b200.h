@@ -250,6 +250,92 @@ int ra_flash_decoding(const ra_dense_params* p);
 size_t ra_flash_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                 int32_t num_tokens, int32_t num_splits);
 
+/* ---- quantised caches and shared prefixes (no counterpart in the reference, whose caches are fp16
+ * and whose batch rows share either everything or nothing) ---- */
+#define RA_TYPE_FP16 0
+#define RA_TYPE_BF16 1
+
+#define RA_CACHE_FP16 0
+#define RA_CACHE_BF16 1
+#define RA_CACHE_INT8 2   /* code = rne(x / s), s = amax / 127 over the row's 128 values */
+#define RA_CACHE_FP8 3    /* e4m3(x / s), s the least power of two with amax <= 448 s */
+#define RA_CACHE_INT4 4   /* code = rne(x / s) + 8, s = amax / 7 over each 32 values; two codes in a
+                             byte, the even value in the low half */
+
+/* A key/value cache of any format: one cache for all batch rows (batch strides 0) or one for each.
+ * Row of token n, head h: 128 elements (int4: 64 bytes) at n*token_stride + h*head_stride.  Its
+ * scales (NULL for fp16 and bf16): 1 float (int4: 4) at h*scale_head_stride + n (int4: + 4n).
+ * Pointers of k and v are 16-byte aligned and the strides are multiples of 16 bytes; scales are
+ * 4-byte (int4: 16-byte) aligned. */
+typedef struct ra_kv_cache {
+  void* k;
+  void* v;                       /* same strides as k */
+  float* k_scale;
+  float* v_scale;
+  int32_t format;                /* RA_CACHE_* */
+  int32_t num_tokens;            /* capacity; 0 = no such cache */
+  int64_t batch_stride;          /* elements (int4: bytes) between two batch rows' caches; 0 = shared */
+  int64_t token_stride;
+  int64_t head_stride;
+  int64_t scale_batch_stride;    /* floats */
+  int64_t scale_head_stride;
+} ra_kv_cache;
+
+/* Rows that go into a quantised cache, or come back out of it.  Row (c, t, h), 128 values of row_type,
+ * belongs to token position_c + t of cache c. */
+typedef struct ra_kv_rows_params {
+  ra_kv_cache cache;             /* format int8, fp8 or int4 */
+  int32_t caches;                /* batch rows with a cache of their own, or 1 */
+  int32_t num_kv_heads, head_dim;
+  void* k_rows;                  /* 16-byte aligned, strides multiples of 8 elements */
+  void* v_rows;
+  int32_t row_type;              /* RA_TYPE_* */
+  int32_t num_rows;              /* per cache */
+  int64_t k_batch_stride, k_token_stride, k_head_stride;   /* elements */
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  const int32_t* positions;      /* optional device int32 [caches]: first token of each cache */
+  int32_t position;              /* first token of every cache when positions is NULL */
+  const int32_t* counts;         /* append only, optional device int32 [caches]: only the first
+                                    counts[c] rows are written (a padded batch) */
+  void* status;                  /* status block, 256 bytes, zeroed once */
+  void* stream;
+} ra_kv_rows_params;
+
+/* Write the rows into the cache.  Everything else in the cache stays as it was.  A token outside
+ * [0, num_tokens) is not written and sets a bit of the status block (RA_ERR_DEVICE_CHECK).  A row (int4: a group of
+ * 32) whose largest magnitude is below 2^-100 is stored as zeros; one with an infinity or a NaN gets
+ * a NaN scale and reads back as NaN. */
+int ra_kv_append_quantized(const ra_kv_rows_params* p);
+/* Read rows back: code * scale, rounded to row_type.  Tokens outside the cache give zeros and set the
+ * status bit; counts is not read. */
+int ra_kv_dequantize(const ra_kv_rows_params* p);
+
+/* Decode attention, one query token per batch row, over a prefix that all rows share followed by each
+ * row's own cache:
+ *   out[b,h] = softmax(sm_scale * q[b,h] . [K_prefix; K_b]) [V_prefix; V_b]
+ * where K_b, V_b are the first seq_lens[b] tokens of row b's cache.  Either part may be absent
+ * (num_tokens 0).  The prefix is read once for all rows, not once for each.  Lengths are clamped to
+ * [0, num_tokens] (one outside sets a bit of the status block); a row with nothing to attend to
+ * gives zeros.  Tokens behind a row's length are not looked at, whatever they hold. */
+typedef struct ra_cache_attention_params {
+  const void* q;                 /* [batch, num_q_heads, 128] of `type`, contiguous */
+  void* out;                     /* same shape and type */
+  int32_t type;                  /* RA_TYPE_*; fp16 and bf16 caches must be of the same type */
+  int32_t batch, num_q_heads, num_kv_heads, head_dim;
+  ra_kv_cache prefix;            /* one cache for all rows (batch strides ignored) */
+  ra_kv_cache cache;             /* one for each row; of the prefix's format when both are given */
+  const int32_t* seq_lens;       /* optional device int32 [batch]; NULL: all rows are num_tokens long */
+  float sm_scale;
+  void* workspace;               /* scratch, 256-byte aligned, never needs zeroing */
+  size_t workspace_bytes;        /* ra_cache_attention_workspace_bytes() */
+  void* status;                  /* status block, 256 bytes, zeroed once */
+  void* stream;
+} ra_cache_attention_params;
+
+size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                          int32_t prefix_tokens, int32_t cache_tokens);
+int ra_cache_attention(const ra_cache_attention_params* p);
+
 /* ---- sequence-sharded decode (no counterpart in the reference, which is single-device) ----
  * The token axis is cut over ranks.  Per step every rank (1) calls ra_gemv_topk on its shard
  * with index_base = first global token id of the shard, (2) all-gathers the [B,Hq,k] score and

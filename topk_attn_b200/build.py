@@ -24,7 +24,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 TUNING_LIB = os.path.join(LIBDIR, "libtopk_attn_b200_tuning.so")
 CU_SOURCES = ["api.cu", "scan_select.cu", "scan_store.cu", "select_stored.cu", "select_sharded.cu", "merge_attend.cu",
-              "gather_attend.cu", "flash_decode.cu", "center_select.cu", "dense_select.cu", "exchange.cu"]
+              "gather_attend.cu", "flash_decode.cu", "center_select.cu", "dense_select.cu", "exchange.cu",
+              "quant_cache.cu", "cache_attend.cu", "cache_api.cu"]
 # sources that read the route / phase overrides when compiled with -DRA_TUNING
 TUNING_SOURCES = ["api.cu", "scan_select.cu", "select_stored.cu", "select_sharded.cu", "dense_select.cu", "center_select.cu", "merge_attend.cu"]
 
@@ -36,10 +37,11 @@ def _newer(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _all_deps():
+def _header_deps():
+    """What every object depends on beside its own source."""
     deps = [os.path.join(ROOT, "include", "topk_attn_b200.h")]
     for f in os.listdir(CSRC):
-        if f.endswith((".cu", ".cuh", ".cpp", ".h")):
+        if f.endswith((".cuh", ".h")):
             deps.append(os.path.join(CSRC, f))
     return deps
 
@@ -50,7 +52,7 @@ def _compile(sources, objdir, extra, deps, force, verbose):
     for src in sources:
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
         objs.append(obj)
-        if force or _newer(obj, deps):
+        if force or _newer(obj, deps + [os.path.join(CSRC, src)]):
             cmd = [NVCC, *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", *extra,
                    "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c",
                    os.path.join(CSRC, src), "-o", obj]
@@ -68,7 +70,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     phase overrides (RA_FORCE_*, RA_NO_*, RA_DEBUG_FLAGS) compiled in, for A/B tests and the
     bench's phase profile.  The default library reads no such variable."""
     os.makedirs(LIBDIR, exist_ok=True)
-    deps = _all_deps()
+    deps = _header_deps()
     objs, fresh = _compile(CU_SOURCES, os.path.join(PKG, "build"), [], deps, force, verbose)
     if force or fresh or _newer(LIB, objs):
         subprocess.check_call([NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-cudart", "static"])

@@ -21,6 +21,9 @@ RA_ERR_CUDA = 4
 RA_ERR_DEVICE_TIMEOUT = 5
 RA_ERR_DEVICE_CHECK = 7
 
+RA_TYPE_FP16, RA_TYPE_BF16 = 0, 1
+RA_CACHE_FP16, RA_CACHE_BF16, RA_CACHE_INT8, RA_CACHE_FP8, RA_CACHE_INT4 = range(5)
+
 
 class RaParams(C.Structure):
     """Mirror of ``struct ra_params``."""
@@ -115,6 +118,41 @@ class RaDenseParams(C.Structure):
     ]
 
 
+class RaKvCache(C.Structure):
+    """Mirror of ``struct ra_kv_cache``."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("format", C.c_int32), ("num_tokens", C.c_int32),
+        ("batch_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("scale_batch_stride", C.c_int64), ("scale_head_stride", C.c_int64),
+    ]
+
+
+class RaKvRowsParams(C.Structure):
+    """Mirror of ``struct ra_kv_rows_params``."""
+    _fields_ = [
+        ("cache", RaKvCache), ("caches", C.c_int32),
+        ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("k_rows", C.c_void_p), ("v_rows", C.c_void_p), ("row_type", C.c_int32), ("num_rows", C.c_int32),
+        ("k_batch_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_batch_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("positions", C.c_void_p), ("position", C.c_int32), ("counts", C.c_void_p),
+        ("status", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class RaCacheAttentionParams(C.Structure):
+    """Mirror of ``struct ra_cache_attention_params``."""
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("type", C.c_int32),
+        ("batch", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("prefix", RaKvCache), ("cache", RaKvCache), ("seq_lens", C.c_void_p), ("sm_scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
 class RaTwoLevelParams(C.Structure):
     """Mirror of ``struct ra_two_level_params``."""
     _fields_ = [
@@ -196,6 +234,10 @@ def _declare(l: C.CDLL) -> None:
                                    C.c_int64, vp, i32, i32, vp]),
         "ra_two_level_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
         "ra_flash_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
+        "ra_kv_append_quantized": (C.c_int, [C.POINTER(RaKvRowsParams)]),
+        "ra_kv_dequantize": (C.c_int, [C.POINTER(RaKvRowsParams)]),
+        "ra_cache_attention": (C.c_int, [C.POINTER(RaCacheAttentionParams)]),
+        "ra_cache_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
         "ra_center_only_topk": (C.c_int, [C.POINTER(RaCenterParams)]),
         "ra_center_workspace_bytes": (sz, [i32, i32, i32, i32]),
         "ra_lse_combine": (C.c_int, [vp, i32, i32, vp, vp]),

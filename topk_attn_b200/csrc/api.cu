@@ -11,6 +11,7 @@
 #include <string>
 #include <tuple>
 
+#include "api_host.cuh"
 #include "center_select.cuh"
 #include "dense_select.cuh"
 #include "exchange.cuh"
@@ -56,11 +57,6 @@ int unsupported(const char* why) {
   g_last_error = why;
   return RA_ERR_UNSUPPORTED;
 }
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = [] {
@@ -108,6 +104,22 @@ int sm_count() {
   }
   return cached[dev];
 }
+
+}  // namespace
+
+namespace ra {
+
+int host_fail(int status, const char* why) {
+  g_last_error = why;
+  return status;
+}
+int host_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int host_sm_count() { return sm_count(); }
+EncodeTiledFn host_encode_fn() { return encode_fn(); }
+
+}  // namespace ra
+
+namespace {
 
 // Parameters of the planner's time model: what the whole device and one multiprocessor stream from
 // HBM.  They rank launch geometries against each other; absolute accuracy is not needed.
@@ -914,9 +926,10 @@ int ra_check_status(void* workspace, void* stream) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "ra_check_status");
   if (h & ra::kStatusTimeout) return RA_ERR_DEVICE_TIMEOUT;
-  if (h & (ra::kStatusBadId | ra::kStatusOverflow)) {
-    g_last_error = (h & ra::kStatusBadId) ? "a kernel skipped a key id outside the value cache"
-                                          : "a candidate list overflowed";
+  if (h & (ra::kStatusBadId | ra::kStatusOverflow | ra::kStatusBadToken)) {
+    g_last_error = (h & ra::kStatusBadId)      ? "a kernel skipped a key id outside the value cache"
+                   : (h & ra::kStatusOverflow) ? "a candidate list overflowed"
+                                               : "a position or length outside a cache was left out or clamped";
     return RA_ERR_DEVICE_CHECK;
   }
   return RA_OK;

@@ -1,0 +1,19 @@
+// What the host sources of the C ABI share: the error text of the calling thread, the device's
+// multiprocessor count and the driver's tensor-map encoder (defined in api.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace ra {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int host_fail(int status, const char* why);             // records the text, returns the status
+int host_cuda_fail(cudaError_t e, const char* what);    // RA_ERR_CUDA with the runtime's text
+int host_sm_count();                                    // of the current device
+EncodeTiledFn host_encode_fn();                         // null where the driver has none
+
+}  // namespace ra

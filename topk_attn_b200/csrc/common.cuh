@@ -29,6 +29,7 @@ constexpr unsigned long long kWaitLimitNs = 1000000000ull;   // bounded mbarrier
 constexpr unsigned kStatusTimeout = 1u;
 constexpr unsigned kStatusBadId = 2u;      // a winner id outside the value cache was skipped
 constexpr unsigned kStatusOverflow = 4u;   // a candidate list overflowed its capacity
+constexpr unsigned kStatusBadToken = 8u;   // a position or length outside a cache was left out or clamped
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -7,7 +7,8 @@ sm_100a kernels.  Layouts are the reference's: q [B,Hq,128], k/v [N,Hkv,128] (sh
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Optional, Tuple
+import dataclasses
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -271,6 +272,290 @@ def kv_append(k_cache: Tensor, v_cache: Tensor, new_k: Tensor, new_v: Tensor, po
         _stream_ptr()))
 
 
+@dataclasses.dataclass
+class QuantizedKV:
+    """A key/value cache held in 8 or 4 bits: one cache for each batch row, or one shared by all.
+
+    * ``k``, ``v``: codes [B,N,Hkv,128] ([N,Hkv,128] shared) int8 or float8_e4m3fn, or uint8
+      [..,N,Hkv,64] for 4 bits (the even value in the low half of a byte, each code plus 8);
+    * ``k_scale``, ``v_scale``: fp32 [B,Hkv,N] ([Hkv,N]), for 4 bits [B,Hkv,N,4] ([Hkv,N,4]).
+
+    ``quantized_kv_cache`` makes an empty one; views along the tokens (``first``) work as caches too."""
+    k: Tensor
+    v: Tensor
+    k_scale: Tensor
+    v_scale: Tensor
+
+    @property
+    def kind(self) -> str:
+        return {torch.int8: "int8", torch.float8_e4m3fn: "fp8", torch.uint8: "int4"}[self.k.dtype]
+
+    @property
+    def per_row(self) -> bool:
+        return self.k.dim() == 4
+
+    @property
+    def num_tokens(self) -> int:
+        return self.k.size(-3)
+
+    def first(self, tokens: int) -> "QuantizedKV":
+        """The cache's first ``tokens`` tokens (a view)."""
+        if not 0 <= tokens <= self.num_tokens:
+            raise ValueError("more tokens than the cache holds")
+        d = -2 if self.kind == "int4" else -1
+        return QuantizedKV(self.k.narrow(-3, 0, tokens), self.v.narrow(-3, 0, tokens),
+                           self.k_scale.narrow(d, 0, tokens), self.v_scale.narrow(d, 0, tokens))
+
+
+def quantized_kv_cache(num_tokens: int, num_kv_heads: int, kind: str = "int8", batch: Optional[int] = None,
+                       device: Union[str, torch.device] = "cuda") -> QuantizedKV:
+    """An empty cache of ``kind`` "int8", "fp8" (e4m3) or "int4" for ``num_tokens`` tokens: one for
+    each of ``batch`` rows, or one shared cache when ``batch`` is None."""
+    if kind not in ("int8", "fp8", "int4"):
+        raise ValueError("kind must be int8, fp8 or int4")
+    if num_tokens < 0 or num_kv_heads < 1 or (batch is not None and batch < 1):
+        raise ValueError("sizes must be positive")
+    lead = () if batch is None else (batch,)
+    dtype = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, "int4": torch.uint8}[kind]
+    codes = (*lead, num_tokens, num_kv_heads, 64 if kind == "int4" else 128)
+    scales = (*lead, num_kv_heads, num_tokens) + ((4,) if kind == "int4" else ())
+    return QuantizedKV(*(torch.zeros(codes, dtype=torch.uint8, device=device).view(dtype) for _ in range(2)),
+                       *(torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+_ROW_TYPES = {torch.float16: capi.RA_TYPE_FP16, torch.bfloat16: capi.RA_TYPE_BF16}
+_CODE_FORMATS = {torch.int8: capi.RA_CACHE_INT8, torch.float8_e4m3fn: capi.RA_CACHE_FP8,
+                 torch.uint8: capi.RA_CACHE_INT4}
+_status_blocks: Dict[int, Tensor] = {}
+
+
+def _status_block(device: torch.device) -> Tensor:
+    """The zeroed status block of ``device`` that ``check_status`` reads.  A graph captured before any
+    eager call on the device gets a block of its own, which ``check_status`` does not see."""
+    st = _status_blocks.get(device.index)
+    if st is None:
+        st = torch.zeros(256, dtype=torch.uint8, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()   # other streams use it from now on
+            _status_blocks[device.index] = st
+    return st
+
+
+def _scratch(nbytes: int, device: torch.device) -> Tensor:
+    """Scratch for one call: the stream's cached workspace behind its status block, or memory of its
+    own inside a capture (two captured graphs may be replayed at the same time, on any streams)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return workspace(nbytes + 256, device)[256:]
+
+
+def _dense_strides(t: Tensor, row: int) -> Tuple[int, int, int]:
+    """(batch, token, head) strides of rows [B,T,H,row] or [T,H,row]; dimensions of size one, whose
+    stride means nothing, get the one a dense tensor would have."""
+    if t.stride(-1) != 1 and t.size(-1) != 1:
+        raise ValueError("the last dimension must be contiguous")
+    hs = t.stride(-2) if t.size(-2) > 1 else row
+    ts = t.stride(-3) if t.size(-3) > 1 else max(t.size(-2) * hs, row)
+    if t.dim() == 4 and t.size(0) > 1:
+        return t.stride(0), ts, hs
+    return max(t.size(-3), 1) * ts, ts, hs
+
+
+def _kv_cache(cache, per_row: bool, device: torch.device) -> Tuple[capi.RaKvCache, int, int]:
+    """(struct, caches, kv heads) of a QuantizedKV or a pair of fp16/bf16 tensors."""
+    c = capi.RaKvCache()
+    quantized = isinstance(cache, QuantizedKV)
+    k, v = (cache.k, cache.v) if quantized else cache
+    if k.dim() != (4 if per_row else 3) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must be [B,N,Hkv,128]" if per_row else "k and v must be [N,Hkv,128]")
+    if quantized:
+        if k.dtype not in _CODE_FORMATS:
+            raise ValueError("codes must be int8, float8_e4m3fn or uint8 (two int4)")
+        c.format = _CODE_FORMATS[k.dtype]
+    else:
+        if k.dtype not in _ROW_TYPES:
+            raise ValueError("caches must be fp16, bf16 or a QuantizedKV")
+        c.format = _ROW_TYPES[k.dtype]
+    int4 = c.format == capi.RA_CACHE_INT4
+    row = 64 if int4 else 128
+    if k.size(-1) != row:
+        raise ValueError(f"rows of this cache must have {row} elements")
+    caches, n, heads = (k.size(0) if per_row else 1), k.size(-3), k.size(-2)
+    for t in (k, v) + ((cache.k_scale, cache.v_scale) if quantized else ()):
+        if t.device != device:
+            raise ValueError("tensors must be on one CUDA device")
+    c.num_tokens = n
+    if n == 0:
+        return c, caches, heads
+    c.batch_stride, c.token_stride, c.head_stride = _dense_strides(k, row)
+    if _dense_strides(v, row) != (c.batch_stride, c.token_stride, c.head_stride):
+        raise ValueError("k and v must have the same strides")
+    c.k, c.v = k.data_ptr(), v.data_ptr()
+    if quantized:
+        ks, vs = cache.k_scale, cache.v_scale
+        want = ((caches,) if per_row else ()) + (heads, n) + ((4,) if int4 else ())
+        for t in (ks, vs):
+            if t.dtype != torch.float32 or tuple(t.shape) != want:
+                raise ValueError(f"scales must be fp32 {list(want)}")
+            if (n > 1 and t.stride(-2 if int4 else -1) != (4 if int4 else 1)) or (int4 and t.stride(-1) != 1):
+                raise ValueError("a head's scales must be contiguous along the tokens")
+
+        def lead(t):
+            hd = 1 if per_row else 0
+            hs = t.stride(hd) if heads > 1 else n * (4 if int4 else 1)
+            return (t.stride(0) if per_row and caches > 1 else heads * hs), hs
+        c.scale_batch_stride, c.scale_head_stride = lead(ks)
+        if lead(vs) != lead(ks):
+            raise ValueError("the scales of k and v must have the same strides")
+        c.k_scale, c.v_scale = ks.data_ptr(), vs.data_ptr()
+    return c, caches, heads
+
+
+def _int32_vector(t: Tensor, n: int, device: torch.device, name: str) -> int:
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on the device of the others")
+    return t.data_ptr()
+
+
+def _kv_rows(cache: QuantizedKV, k: Tensor, v: Tensor, position, counts: Optional[Tensor]) -> capi.RaKvRowsParams:
+    dev = k.device
+    p = capi.RaKvRowsParams()
+    p.cache, p.caches, p.num_kv_heads = _kv_cache(cache, cache.per_row, dev)
+    if k.dim() != cache.k.dim() or k.size(-1) != 128 or k.size(-2) != p.num_kv_heads or v.shape != k.shape \
+            or (cache.per_row and k.size(0) != p.caches):
+        raise ValueError("rows must be [B,T,Hkv,128] for per-row caches, [T,Hkv,128] for a shared one")
+    if k.dtype not in _ROW_TYPES or v.dtype != k.dtype or v.device != dev:
+        raise ValueError("rows must be fp16 or bf16 tensors on the device of the cache")
+    p.head_dim, p.row_type, p.num_rows = 128, _ROW_TYPES[k.dtype], k.size(-3)
+    p.k_batch_stride, p.k_token_stride, p.k_head_stride = _dense_strides(k, 128)
+    p.v_batch_stride, p.v_token_stride, p.v_head_stride = _dense_strides(v, 128)
+    p.k_rows, p.v_rows = k.data_ptr(), v.data_ptr()
+    if isinstance(position, Tensor):
+        p.positions = _int32_vector(position, p.caches, dev, "position")
+    else:
+        p.position = int(position)
+    if counts is not None:
+        p.counts = _int32_vector(counts, p.caches, dev, "counts")
+    p.status, p.stream = _status_block(dev).data_ptr(), _stream_ptr()
+    return p
+
+
+def kv_append_quantized(cache: QuantizedKV, new_k: Tensor, new_v: Tensor, position: Union[int, Tensor],
+                        counts: Optional[Tensor] = None) -> None:
+    """In place: quantise the rows new_k, new_v (fp16 or bf16 [B,T,Hkv,128]; [T,Hkv,128] for a shared
+    cache; any strides with contiguous rows of 16-byte alignment, so views of a fused projection
+    do) and store them as the tokens position .. position+T-1 of each cache.
+
+    ``position`` is one int for all caches or an int32 tensor [B] ([1] for a shared cache) on the
+    device; ``counts`` int32 [B] says how many of the T rows of each are written (a padded batch).
+    Rows that a device-side position puts outside the cache are left out and reported by
+    ``check_status``."""
+    if not new_k.is_cuda:
+        raise ValueError("tensors must be CUDA tensors")
+    if new_k.dim() >= 3 and new_k.size(-3) == 0:
+        return
+    with torch.cuda.device(new_k.device):
+        capi.check(capi.lib().ra_kv_append_quantized(C.byref(_kv_rows(cache, new_k, new_v, position, counts))))
+
+
+def kv_dequantize(cache: QuantizedKV, position: Union[int, Tensor] = 0, count: Optional[int] = None,
+                  dtype: torch.dtype = torch.float16) -> Tuple[Tensor, Tensor]:
+    """The values held for the tokens position .. position+count-1 of each cache, as fp16 or bf16
+    tensors [B,count,Hkv,128] ([count,Hkv,128] for a shared cache).  ``position`` is as in
+    ``kv_append_quantized``; ``count`` defaults to all tokens behind an int position.  Tokens that a
+    device-side position puts outside the cache read as zeros and are reported by ``check_status``."""
+    if dtype not in _ROW_TYPES:
+        raise ValueError("dtype must be float16 or bfloat16")
+    if not cache.k.is_cuda:
+        raise ValueError("tensors must be CUDA tensors")
+    if count is None:
+        if isinstance(position, Tensor):
+            raise ValueError("a position on the device needs a count")
+        count = cache.num_tokens - position
+    if count < 0:
+        raise ValueError("count must not be negative")
+    shape = (*cache.k.shape[:-3], count, cache.k.size(-2), 128)
+    with torch.cuda.device(cache.k.device):
+        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        if count:
+            capi.check(capi.lib().ra_kv_dequantize(C.byref(_kv_rows(cache, k, v, position, None))))
+    return k, v
+
+
+def _cache_attention(q: Tensor, prefix, cache, sm_scale: float, seq_lens: Optional[Tensor],
+                     out: Optional[Tensor]) -> Tensor:
+    if not q.is_cuda:
+        raise ValueError("tensors must be CUDA tensors")
+    if q.dim() != 3 or q.size(2) != 128 or q.dtype not in _ROW_TYPES or not q.is_contiguous():
+        raise ValueError("q must be a contiguous fp16 or bf16 tensor [B,Hq,128]")
+    dev = q.device
+    B, Hq, _ = q.shape
+    if prefix is None and cache is None:
+        raise ValueError("nothing to attend to: give a prefix, a cache or both")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of the shape and type of q")
+    with torch.cuda.device(dev):
+        p = capi.RaCacheAttentionParams()
+        p.q, p.out, p.type = q.data_ptr(), out.data_ptr(), _ROW_TYPES[q.dtype]
+        p.batch, p.num_q_heads, p.head_dim = B, Hq, 128
+        heads = []
+        if prefix is not None:
+            p.prefix, _, h = _kv_cache(prefix, False, dev)
+            heads.append(h)
+        if cache is not None:
+            p.cache, caches, h = _kv_cache(cache, True, dev)
+            heads.append(h)
+            if caches != B:
+                raise ValueError("each row needs a cache: cache.size(0) must be the batch")
+        if len(set(heads)) != 1:
+            raise ValueError("prefix and cache must have the same kv heads")
+        p.num_kv_heads = heads[0]
+        if seq_lens is not None:
+            if cache is None:
+                raise ValueError("seq_lens are the lengths of the rows' own caches")
+            p.seq_lens = _int32_vector(seq_lens, B, dev, "seq_lens")
+        p.sm_scale = sm_scale
+        need = capi.lib().ra_cache_attention_workspace_bytes(B, Hq, p.num_kv_heads, p.prefix.num_tokens,
+                                                             p.cache.num_tokens)
+        ws = _scratch(max(need, 256), dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        p.status, p.stream = _status_block(dev).data_ptr(), _stream_ptr()
+        capi.check(capi.lib().ra_cache_attention(C.byref(p)))
+    return out
+
+
+def flash_decoding_quantized(q: Tensor, cache: QuantizedKV, sm_scale: float, seq_lens: Optional[Tensor] = None,
+                             out: Optional[Tensor] = None) -> Tensor:
+    """Dense decode attention that reads a quantised cache as it is held.  q fp16 or bf16 [B,Hq,128];
+    ``cache`` holds one cache for each row (``seq_lens`` int32 [B] on the device: how many of its tokens
+    each row sees, all when None) or one shared by all rows (``cache.first(n)`` for a part of it).
+    Returns [B,Hq,128] of q's type; a row that sees nothing gets zeros."""
+    if not isinstance(cache, QuantizedKV):
+        raise ValueError("cache must be a QuantizedKV")
+    if cache.per_row:
+        return _cache_attention(q, None, cache, sm_scale, seq_lens, out)
+    if seq_lens is not None:
+        raise ValueError("a shared cache has one length: give cache.first(length)")
+    return _cache_attention(q, cache, None, sm_scale, None, out)
+
+
+KVCache = Union[QuantizedKV, Tuple[Tensor, Tensor]]
+
+
+def shared_prefix_attention(q: Tensor, prefix: Optional[KVCache], cache: Optional[KVCache], sm_scale: float,
+                            seq_lens: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """Decode attention of rows whose sequences start with one common prefix: softmax over the prefix's
+    keys followed by the row's own, in one normalisation, with the prefix read once for all rows.
+
+    q fp16 or bf16 [B,Hq,128]; ``prefix`` (k, v) [Np,Hkv,128] of q's type or a shared QuantizedKV;
+    ``cache`` (k, v) [B,N,Hkv,128] or a per-row QuantizedKV of the same kind; either may be None.
+    ``seq_lens`` int32 [B] on the device: how many tokens of its own cache each row sees (all when
+    None; 0: the prefix only).  Returns [B,Hq,128] of q's type; a row that sees nothing gets zeros."""
+    return _cache_attention(q, prefix, cache, sm_scale, seq_lens, out)
+
+
 def merge_attend(cand_scores: Tensor, cand_indices: Tensor, v: Tensor, topk: int, sm_scale: float,
                  own_base: int, partial: bool = True, return_indices: bool = False,
                  out: Optional[Tensor] = None, exchange=None, own_part: Optional[int] = None):
@@ -434,3 +719,15 @@ def check_status(device: Optional[torch.device] = None) -> None:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     ws = workspace(256, dev)
     capi.check(capi.lib().ra_check_status(ws.data_ptr(), _stream_ptr()))
+    st = _status_blocks.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    if st is not None:
+        capi.check(capi.lib().ra_check_status(st.data_ptr(), _stream_ptr()))
+
+
+def clear_status(device: Optional[torch.device] = None) -> None:
+    """Reset the sticky bits that ``check_status`` reports, in order of the current stream."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    workspace(256, dev)[:256].zero_()
+    st = _status_blocks.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    if st is not None:
+        st.zero_()
