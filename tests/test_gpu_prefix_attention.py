@@ -52,7 +52,9 @@ def check(q, prefix, own, kind, lens=None, dtype=None, call=None):
     tol = O.tolerance(ref, q, SM, [p[0] for p in parts if p[0].numel()], [p[1] for p in parts if p[1].numel()], total,
                       q.dtype, kind)
     far = (out.cpu().double() - ref).abs()
-    assert out.dtype == q.dtype and (far <= tol).all(), float((far / tol).max())
+    assert out.dtype == q.dtype
+    worst = float((far / tol).max())
+    assert worst <= 1.0
     return out
 
 

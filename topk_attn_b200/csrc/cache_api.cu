@@ -2,6 +2,7 @@
 // validation and launches.  Nothing here allocates device memory or synchronises.
 #include "topk_attn_b200.h"
 
+#include <cstdio>
 #include <cstring>
 
 #include <algorithm>
@@ -88,12 +89,56 @@ int check_rows(const ra_kv_rows_params* p, QuantParams& q) {
   return RA_OK;
 }
 
-// splits of one segment's tokens: about eight CTAs per multiprocessor, 256 tokens each at least
-int split_count(int batch, int hq, int n) {
-  if (n <= 0) return 0;
-  const long long rows = (long long)batch * hq;
-  const long long want = std::max<long long>(1, 8 * 148 / rows);
-  return (int)std::min<long long>(want, (n + 255) / 256);
+// Tensor map over K or V: 64-token boxes of one head, swizzled over the 128 (int4: 64) bytes of a row.
+int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int format, int heads, int caches) {
+  EncodeTiledFn enc = host_encode_fn();
+  if (!enc) return host_fail(RA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const bool dense = format <= RA_CACHE_BF16;
+  const cuuint64_t row = dense ? kHeadDim : cache_row_bytes(format);
+  const cuuint64_t dims[4] = {row, (cuuint64_t)heads, (cuuint64_t)v.n_tokens, (cuuint64_t)caches};
+  const cuuint64_t strides[3] = {(cuuint64_t)v.hstride, (cuuint64_t)v.tstride,
+                                 (cuuint64_t)(caches > 1 ? v.bstride : v.tstride)};
+  const cuuint32_t box[4] = {(cuuint32_t)(dense ? 64 : row), 1, (cuuint32_t)kAttendTile, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = format == RA_CACHE_FP16   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : format == RA_CACHE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUresult r = enc(map, type, 4, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         format == RA_CACHE_INT4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return RA_OK;
+  char buf[96];
+  snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return host_fail(RA_ERR_CUDA, buf);
+}
+
+// How one segment is worked on, and where its partials lie in the scratch.
+struct SegmentPlan {
+  int caches, queries, nq, query_tiles, grid;
+  size_t ml_at, line_at, bytes;   // part_o at 0
+};
+
+constexpr int kMaxSms = 256;      // bound of the device-independent workspace size
+
+SegmentPlan plan_segment(bool prefix, int batch, int hq, int hkv, int tokens, int sms) {
+  SegmentPlan s;
+  memset(&s, 0, sizeof s);
+  if (tokens <= 0) return s;
+  const int group = hq / hkv;
+  s.caches = prefix ? 1 : batch;
+  s.queries = prefix ? batch * group : group;
+  s.nq = s.queries <= 8 ? 1 : 2;
+  s.query_tiles = (s.queries + 8 * s.nq - 1) / (8 * s.nq);
+  const long long rows = (long long)s.caches * hkv * s.query_tiles;
+  const long long tiles = rows * ((tokens + kAttendTile - 1) / kAttendTile);
+  s.grid = (int)std::min<long long>(tiles, (long long)attend_ctas(s.nq) * sms);
+  const size_t slots = (size_t)rows + s.grid;
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  s.ml_at = up(slots * 8 * s.nq * kHeadDim * sizeof(float));
+  s.line_at = s.ml_at + up(slots * 8 * s.nq * 2 * sizeof(float));
+  s.bytes = s.line_at + up((size_t)(s.caches + 1) * sizeof(long long));
+  return s;
 }
 
 }  // namespace
@@ -126,11 +171,9 @@ int ra_kv_dequantize(const ra_kv_rows_params* p) {
 
 size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                           int32_t prefix_tokens, int32_t cache_tokens) {
-  if (batch < 1 || num_kv_heads < 1 || num_q_heads < 1 || prefix_tokens < 0 || cache_tokens < 0) return 0;
-  const size_t rows = (size_t)batch * num_q_heads;
-  const size_t parts = (size_t)split_count(batch, num_q_heads, prefix_tokens) +
-                       (size_t)split_count(batch, num_q_heads, cache_tokens);
-  return std::max<size_t>(256, rows * parts * kPartialFloats * sizeof(float));
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || prefix_tokens < 0 || cache_tokens < 0) return 0;
+  return 256 + plan_segment(true, batch, num_q_heads, num_kv_heads, prefix_tokens, kMaxSms).bytes +
+         plan_segment(false, batch, num_q_heads, num_kv_heads, cache_tokens, kMaxSms).bytes;
 }
 
 int ra_cache_attention(const ra_cache_attention_params* p) {
@@ -146,25 +189,14 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   if (p->prefix.num_tokens < 0 || p->cache.num_tokens < 0) return invalid("sizes must not be negative");
   if (has[0] && has[1] && p->prefix.format != p->cache.format)
     return invalid("prefix and cache must have one format");
-  if ((long long)p->batch * p->num_q_heads > 65535) return unsupported("more than 65535 query rows");
-  CacheAttendParams c[2];
+  if ((long long)p->batch * p->num_q_heads > (1 << 24)) return unsupported("more than 2^24 query rows");
+  CacheView view[2];
   for (int i = 0; i < 2; ++i) {
     const ra_kv_cache& kv = i ? p->cache : p->prefix;
-    memset(&c[i], 0, sizeof c[i]);
     if (!has[i]) continue;
     if (kv.format <= RA_CACHE_BF16 && kv.format != p->type) return invalid("the cache must have the type of q");
-    const int st = view_of(kv, i == 1, p->batch, c[i].cache);
+    const int st = view_of(kv, i == 1, p->batch, view[i]);
     if (st != RA_OK) return st;
-    c[i].q = p->q;
-    c[i].batch = p->batch;
-    c[i].hq = p->num_q_heads;
-    c[i].hkv = p->num_kv_heads;
-    c[i].group = p->num_q_heads / p->num_kv_heads;
-    c[i].seq_lens = i ? p->seq_lens : nullptr;
-    c[i].status = static_cast<unsigned*>(p->status);
-    c[i].splits = split_count(p->batch, p->num_q_heads, kv.num_tokens);
-    c[i].split_len = (kv.num_tokens + c[i].splits - 1) / c[i].splits;
-    c[i].scale_log2e = p->sm_scale * kLog2e;
   }
   const size_t need = ra_cache_attention_workspace_bytes(p->batch, p->num_q_heads, p->num_kv_heads,
                                                          p->prefix.num_tokens, p->cache.num_tokens);
@@ -173,16 +205,55 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
                      "workspace missing, misaligned or smaller than ra_cache_attention_workspace_bytes()");
   cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const bool bf16 = p->type == RA_TYPE_BF16;
-  const int rows = p->batch * p->num_q_heads;
-  c[0].partials = static_cast<float*>(p->workspace);
-  c[1].partials = c[0].partials + (size_t)c[0].splits * rows * kPartialFloats;
+  const int sms = std::min(host_sm_count(), kMaxSms);
+  CombineParams cp;
+  memset(&cp, 0, sizeof cp);
+  cp.out = p->out;
+  cp.batch = p->batch;
+  cp.hq = p->num_q_heads;
+  cp.hkv = p->num_kv_heads;
+  cp.group = p->num_q_heads / p->num_kv_heads;
+  char* at = static_cast<char*>(p->workspace);
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;
-    const cudaError_t e = launch_cache_attend(c[i], (i ? p->cache : p->prefix).format, bf16, stream);
+    const int format = (i ? p->cache : p->prefix).format;
+    const SegmentPlan s = plan_segment(i == 0, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
+    CacheAttendParams a;
+    memset(&a, 0, sizeof a);
+    AttendSegment& g = a.seg;
+    int st = encode_map(&g.kmap, view[i].k, view[i], format, p->num_kv_heads, s.caches);
+    if (st == RA_OK) st = encode_map(&g.vmap, view[i].v, view[i], format, p->num_kv_heads, s.caches);
+    if (st != RA_OK) return st;
+    g.cache = view[i];
+    g.lens = i ? p->seq_lens : nullptr;
+    g.caches = s.caches;
+    g.queries = s.queries;
+    g.query_tiles = s.query_tiles;
+    g.grid = s.grid;
+    g.nstages = cache_attend_stages(format, s.nq);
+    g.part_o = reinterpret_cast<float*>(at);
+    g.part_ml = reinterpret_cast<float*>(at + s.ml_at);
+    g.line = reinterpret_cast<long long*>(at + s.line_at);
+    a.q = p->q;
+    a.status = static_cast<unsigned*>(p->status);
+    a.hq = p->num_q_heads;
+    a.hkv = p->num_kv_heads;
+    a.group = cp.group;
+    a.scale_log2e = p->sm_scale * kLog2e;
+    CombineSegment& c = cp.seg[i];
+    c.part_o = g.part_o;
+    c.part_ml = g.part_ml;
+    c.line = g.line;
+    c.queries = s.queries;
+    c.query_tiles = s.query_tiles;
+    c.qt = 8 * s.nq;
+    c.grid = s.grid;
+    c.prefix = i == 0;
+    at += s.bytes;
+    const cudaError_t e = launch_cache_attend(a, format, bf16, s.nq, stream);
     if (e != cudaSuccess) return host_cuda_fail(e, "cache_attend launch");
   }
-  const cudaError_t e = launch_cache_combine(c[0].partials, c[0].splits, c[1].partials, c[1].splits, rows, p->out,
-                                             bf16, stream);
+  const cudaError_t e = launch_cache_combine(cp, bf16, stream);
   return e == cudaSuccess ? RA_OK : host_cuda_fail(e, "cache_combine launch");
 }
 

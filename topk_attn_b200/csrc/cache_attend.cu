@@ -1,161 +1,767 @@
 // Decode attention over one segment (a prefix shared by the batch, or each row's own cache) in any
 // of the cache formats, and the joining of the segments' partials.
 //
-// Simple form: one CTA per (batch row, query head, split of the tokens), a warp per token with four
-// dimensions in each lane, online softmax, partials (sums, weight, maximum) joined by their maxima.
+// A tile of 64 tokens arrives by TMA in a ring of stages; four consumer warps take 16 tokens each.
+// Both products run on the tensor cores with the tokens (then the dims) as the 16 rows of
+// m16n8k16 and the queries as its 8 columns, so that a group of up to 8 query heads costs one MMA
+// where the other orientation would pad it to 16:
+//     S^T[token, query] = K Q^T          O^T[dim, query] += V^T P^T
+// Codes become fp16 (every int8, e4m3 and int4 code is exact in it) in registers on the way to the
+// MMA and are multiplied as they are; the scales stay outside in fp32: a token's K scale multiplies its
+// scores, its V scale (relative to the largest seen, a power of two) its weights.  int4 has a scale for
+// each 32 dims: the scores of the four groups are accumulated apart, and the weights multiplied once
+// for each group.  K's dims may go through the MMA in any order, so a lane takes them as they lie in
+// 16 (int4: 4) bytes of a row; V's dims come out in the order the lanes hold them.
+//
+// The running maximum moves only when a score exceeds it by 2^4 (a vote, no reduction).  Weights are
+// exp2(score - maximum + 10), at most 2^14 (2^15 with a V scale): fp32 sums do not mind, and fp16, to
+// which they are rounded for the product (bf16 for a bf16 cache), keeps its eleven bits down to 2^-24
+// of the largest.
+// HBM-bound: 264 bytes per token and kv head in 8 bits, 160 in 4, 512 in 16.
 #include "cache_attend.cuh"
 
 namespace ra {
 
-constexpr int kAttendWarps = 4;
+template <int NQ>
+struct AttendCtrl {
+  uint64_t full[kAttendMaxStages];
+  uint64_t empty[kAttendMaxStages];
+  long long before;                 // tiles before cache `start`
+  long long total;
+  long long sums[kAttendThreads / 32 + 1];
+  float m[kAttendWarps][8 * NQ];
+  float l[kAttendWarps][8 * NQ];
+  float c[kAttendWarps];
+  int start;
+  int timeout;
+};
+constexpr int kMergePitch = 68;     // floats of one query's half row in the merge buffer
+constexpr int kMergeBytes = kAttendWarps * 8 * kMergePitch * 4;
+constexpr float kLazyLog2 = 4.f, kLiftLog2 = 10.f;
 
-template <int FMT>
-__device__ __forceinline__ void load4(const unsigned char* row, const float* scale, int lane, float (&x)[4]) {
-  if (FMT == kCacheFp16 || FMT == kCacheBf16) {
-    const uint2 u = *reinterpret_cast<const uint2*>(row + 8 * lane);
-    if (FMT == kCacheBf16) {
-      x[0] = __uint_as_float(u.x << 16);
-      x[1] = __uint_as_float(u.x & 0xffff0000u);
-      x[2] = __uint_as_float(u.y << 16);
-      x[3] = __uint_as_float(u.y & 0xffff0000u);
-    } else {
-      const float2 a = h2f2(u.x), b = h2f2(u.y);
-      x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-    }
-  } else if (FMT == kCacheInt4) {
-    const uint32_t w = *reinterpret_cast<const uint16_t*>(row + 2 * lane);
-    const float s = scale[lane >> 3];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (float)((int)((w >> (4 * i)) & 15u) - 8) * s;
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * lane);
-    const float s = scale[0];
-    if (FMT == kCacheInt8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i)) * s;
-    } else {
-      uint32_t a, b;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)w));
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(w >> 16)));
-      const float2 f = h2f2(a), g = h2f2(b);
-      x[0] = f.x * s; x[1] = f.y * s; x[2] = g.x * s; x[3] = g.y * s;
-    }
-  }
+__device__ __forceinline__ void attend_consumer_sync() {
+  asm volatile("bar.sync 1, %0;" ::"r"(32 * kAttendWarps) : "memory");
 }
-
-template <int FMT, bool BF16>
-__global__ void __launch_bounds__(32 * kAttendWarps)
-cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
-  __shared__ float sm_o[kAttendWarps][kHeadDim], sm_m[kAttendWarps], sm_l[kAttendWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x, row = blockIdx.y, b = row / P.hq, h = (row % P.hq) / P.group;
-  int len = P.cache.n_tokens;
-  if (P.seq_lens) {
-    const int asked = P.seq_lens[b];
-    if ((asked < 0 || asked > len) && threadIdx.x == 0 && split == 0) atomicOr(P.status, kStatusBadToken);
-    len = max(0, min(len, asked));
-  }
-  const int lo = split * P.split_len, hi = min(len, lo + P.split_len);
-  float q[4];
-  load4<BF16 ? kCacheBf16 : kCacheFp16>(static_cast<const unsigned char*>(P.q) + (size_t)row * kRowBytes, nullptr,
-                                        lane, q);
-  constexpr int kScales = cache_row_scales(FMT);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int t = lo + warp; t < hi; t += kAttendWarps) {
-    const long long at = b * P.cache.bstride + t * P.cache.tstride + h * P.cache.hstride;
-    const long long sat = b * P.cache.sbstride + h * P.cache.shstride + (long long)t * kScales;
-    float k[4], v[4];
-    load4<FMT>(P.cache.k + at, P.cache.k_scale + sat, lane, k);
-    load4<FMT>(P.cache.v + at, P.cache.v_scale + sat, lane, v);
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-    for (int i = 16; i; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-    s *= P.scale_log2e;
-    const float m_new = fmaxf(m, s), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float a = exp2f(m - m_use), p = exp2f(s - m_use);
-    l = l * a + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * a + p * v[i];
-    m = m_new;
-  }
-  if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sm_o[warp][4 * lane + i] = o[i];
-  __syncthreads();
-  float top = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kAttendWarps; ++w) top = fmaxf(top, sm_m[w]);
-  const float use = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, wsum = 0.f;
-#pragma unroll
-  for (int w = 0; w < kAttendWarps; ++w) {
-    const float f = exp2f(sm_m[w] - use);
-    sum += f * sm_o[w][threadIdx.x];
-    wsum += f * sm_l[w];
-  }
-  float* out = P.partials + ((size_t)row * P.splits + split) * kPartialFloats;
-  out[threadIdx.x] = sum;
-  if (threadIdx.x == 0) {
-    out[kHeadDim] = wsum;
-    out[kHeadDim + 1] = top;
-  }
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// out[row] = sum over both segments' partials, joined by their maxima; zeros where nothing was seen.
 template <bool BF16>
-__global__ void __launch_bounds__(kHeadDim)
-cache_combine_kernel(const float* a, int na, const float* b, int nb, void* out) {
-  const int row = blockIdx.x, d = threadIdx.x;
-  float m = -INFINITY;
-  for (int i = 0; i < na + nb; ++i) {
-    const float* p = i < na ? a + ((size_t)row * na + i) * kPartialFloats : b + ((size_t)row * nb + i - na) * kPartialFloats;
-    m = fmaxf(m, p[kHeadDim + 1]);
+__device__ __forceinline__ void mma_any(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16) mma_bf16_16816(d, a, b0, b1);
+  else mma_16816(d, a, b0, b1);
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t r;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ uint32_t hsub2_bits(uint32_t a, uint32_t b) {
+  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// Two pairs of fp16 codes out of the bytes (0,2) and (1,3) of a word.  int8: a byte with its sign bit
+// flipped, put into the low mantissa bits of 1024.0, is 1024 + 128 + code.  e4m3: sign and the
+// seven other bits moved to fp16's places give code * 2^-8 (the exponents' biases differ by 8),
+// subnormals included.
+template <int FMT>
+__device__ __forceinline__ void codes_of(uint32_t w, uint32_t& even, uint32_t& odd) {
+  if (FMT == kCacheInt8) {
+    even = hsub2_bits((w & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+    odd = hsub2_bits(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+  } else {
+    const uint32_t x = w << 8;
+    even = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
+    odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
   }
-  const float use = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, w = 0.f;
-  for (int i = 0; i < na + nb; ++i) {
-    const float* p = i < na ? a + ((size_t)row * na + i) * kPartialFloats : b + ((size_t)row * nb + i - na) * kPartialFloats;
-    const float f = exp2f(p[kHeadDim + 1] - use);
-    sum += f * p[d];
-    w += f * p[kHeadDim];
+}
+// nibbles (i, i + 4) of a word, which hold code + 8
+__device__ __forceinline__ uint32_t nibbles_of(uint32_t w, int i) {
+  return hsub2_bits(((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, 0x64086408u);
+}
+
+// The place in the line of work rows: cache, (kv head, query tile), tile of tokens.
+struct AttendWalk {
+  int b, inner, tile, len, tiles;
+};
+
+template <int FMT, bool BF16, int NQ>
+__global__ void __launch_bounds__(kAttendThreads, attend_ctas(NQ))
+cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
+  constexpr bool kDense = FMT <= kCacheBf16;
+  constexpr bool kPBf16 = kDense && BF16;           // type of the weights in the product
+  constexpr int kHalf = kAttendTile * 128;          // one swizzled [64 tokens][128 bytes] block
+  constexpr int kKBytes = kAttendTile * cache_row_bytes(FMT);
+  constexpr int kStage = 2 * kKBytes;
+  constexpr int QT = 8 * NQ;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const AttendSegment& G = P.seg;
+  const int S = G.nstages;
+  float* sm_o = reinterpret_cast<float*>(smem + (size_t)S * kStage);   // [4 warps][8 queries][68]
+  AttendCtrl<NQ>* ctrl = reinterpret_cast<AttendCtrl<NQ>*>(reinterpret_cast<unsigned char*>(sm_o) + kMergeBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per_cache = P.hkv * G.query_tiles;
+
+  if (tid == 0) {
+    tma_prefetch_desc(&G.kmap);
+    tma_prefetch_desc(&G.vmap);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&ctrl->full[s], 1);
+      mbar_init(&ctrl->empty[s], kAttendWarps);
+    }
+    ctrl->timeout = 0;
+    fence_barrier_init();
   }
-  const float r = w == 0.f ? 0.f : sum / w;
-  if (BF16) static_cast<__nv_bfloat16*>(out)[(size_t)row * kHeadDim + d] = __float2bfloat16_rn(r);
-  else static_cast<__half*>(out)[(size_t)row * kHeadDim + d] = __float2half_rn(r);
+  auto length_of = [&](int b) {
+    int len = G.cache.n_tokens;
+    if (G.lens) len = max(0, min(len, G.lens[b]));
+    return len;
+  };
+  auto tiles_of = [&](int b) { return ceil_div(length_of(b), kAttendTile); };
+
+  // ---- my share of the line: every thread sums a run of caches, a block-wide scan does the rest
+  {
+    const int run = ceil_div(G.caches, kAttendThreads);
+    const int lo = min(G.caches, tid * run), hi = min(G.caches, lo + run);
+    long long mine = 0;
+    for (int b = lo; b < hi; ++b) {
+      mine += tiles_of(b);
+      if (G.lens && blockIdx.x == 0 && (G.lens[b] < 0 || G.lens[b] > G.cache.n_tokens))
+        atomicOr(P.status, kStatusBadToken);
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, i);
+      if (lane >= i) incl += o;
+    }
+    if (lane == 31) ctrl->sums[warp] = incl;
+    __syncthreads();
+    long long base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttendThreads / 32; ++w) {
+      if (w < warp) base += ctrl->sums[w];
+      total += ctrl->sums[w];
+    }
+    long long at = base + incl - mine;          // tiles of one (kv head, query tile) before cache lo
+    const long long all = total * per_cache;
+    const long long ctas = min((long long)G.grid, all);   // every one of them has a tile
+    const long long first = blockIdx.x < ctas ? all * blockIdx.x / ctas : all;
+    for (int b = lo; b < hi; ++b) {
+      const int n = tiles_of(b);
+      if (blockIdx.x == 0) G.line[b] = at;
+      if (first >= at * per_cache && first < (at + n) * per_cache) {
+        ctrl->start = b;
+        ctrl->before = at;
+      }
+      at += n;
+    }
+    if (tid == 0) {
+      ctrl->total = total;
+      if (blockIdx.x == 0) G.line[G.caches] = total;
+    }
+    __syncthreads();
+  }
+  // lets the combine kernel start its launch; it waits for this grid's end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const long long total = ctrl->total * per_cache;
+  const long long ctas = min((long long)G.grid, total);
+  if (blockIdx.x >= ctas) return;
+  const long long t0 = total * blockIdx.x / ctas, t1 = total * (blockIdx.x + 1) / ctas;
+  const int my_tiles = (int)(t1 - t0);
+
+  AttendWalk cur;
+  {
+    cur.b = ctrl->start;
+    cur.len = length_of(cur.b);
+    cur.tiles = ceil_div(cur.len, kAttendTile);
+    const int off = (int)(t0 - ctrl->before * per_cache);
+    cur.inner = off / cur.tiles;
+    cur.tile = off % cur.tiles;
+  }
+  auto advance = [&](AttendWalk& w) {
+    if (++w.tile < w.tiles) return;
+    w.tile = 0;
+    if (++w.inner < per_cache) return;
+    w.inner = 0;
+    do {
+      ++w.b;
+      w.len = w.b < G.caches ? length_of(w.b) : 1;
+      w.tiles = ceil_div(w.len, kAttendTile);
+    } while (w.tiles == 0);
+  };
+
+  if (warp == kAttendWarps) {
+    // ---------------------------------------------------------------- producer warp
+    if (lane == 0) {
+      for (int n = 0; n < my_tiles; ++n) {
+        const int s = n % S;
+        if (n >= S && !mbar_wait(&ctrl->empty[s], (unsigned)(((n / S) - 1) & 1), &ctrl->timeout))
+          atomicOr(P.status, kStatusTimeout);
+        unsigned char* dst = smem + (size_t)s * kStage;
+        const int tok = cur.tile * kAttendTile, h = cur.inner / G.query_tiles;
+        mbar_expect_tx(&ctrl->full[s], kStage);
+        if (kDense) {
+          tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, h, tok, cur.b);
+          tma_load_4d(dst + kHalf, &G.kmap, &ctrl->full[s], 64, h, tok, cur.b);
+          tma_load_4d(dst + 2 * kHalf, &G.vmap, &ctrl->full[s], 0, h, tok, cur.b);
+          tma_load_4d(dst + 3 * kHalf, &G.vmap, &ctrl->full[s], 64, h, tok, cur.b);
+        } else {
+          tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, h, tok, cur.b);
+          tma_load_4d(dst + kKBytes, &G.vmap, &ctrl->full[s], 0, h, tok, cur.b);
+        }
+        advance(cur);
+      }
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumer warps
+  const int g = lane >> 2, t = lane & 3;
+  const int r0 = warp * 16;
+  const uint32_t stage0 = smem_u32(smem);
+  const int mi = lane >> 3, lr = lane & 7;
+  // scales of the next tile, fetched one tile ahead: tokens g and g + 8 of my 16
+  constexpr int kNS = kDense ? 1 : cache_row_scales(FMT);
+  float ks_next[2][kNS], vs_next[2][kNS];
+  auto fetch_scales = [&](const AttendWalk& w) {
+    if (kDense) return;
+    const int h = w.inner / G.query_tiles;
+    const long long base = (long long)w.b * G.cache.sbstride + (long long)h * G.cache.shstride;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tok = w.tile * kAttendTile + r0 + g + 8 * i;
+      const bool live = tok < w.len;
+      const float* kp = G.cache.k_scale + base + (long long)tok * kNS;
+      const float* vp = G.cache.v_scale + base + (long long)tok * kNS;
+      if (kNS == 4) {
+        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = live ? __ldg(reinterpret_cast<const float4*>(kp)) : z;
+        const float4 b = live ? __ldg(reinterpret_cast<const float4*>(vp)) : z;
+        ks_next[i][0] = a.x; ks_next[i][kNS > 1 ? 1 : 0] = a.y; ks_next[i][kNS > 2 ? 2 : 0] = a.z; ks_next[i][kNS - 1] = a.w;
+        vs_next[i][0] = b.x; vs_next[i][kNS > 1 ? 1 : 0] = b.y; vs_next[i][kNS > 2 ? 2 : 0] = b.z; vs_next[i][kNS - 1] = b.w;
+      } else {
+        ks_next[i][0] = live ? __ldg(kp) : 0.f;
+        vs_next[i][0] = live ? __ldg(vp) : 0.f;
+      }
+    }
+  };
+  if (!kDense) fetch_scales(cur);
+  AttendWalk nxt = cur;
+
+  int n = 0;
+  while (n < my_tiles) {
+    // ---- one work row
+    const int b = cur.b, h = cur.inner / G.query_tiles, q0 = (cur.inner % G.query_tiles) * QT;
+    const long long row = (long long)b * per_cache + cur.inner;
+    // B fragments of Q^T: column g is query q0 + 8 nq + g; the dims of lane t in the order K's lanes hold them
+    uint32_t qb[NQ][8][2];
+    float fac[NQ][2];      // what turns a raw score of my two columns into the log2 domain
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      const int qi = q0 + 8 * nq + g;
+      const bool live = qi < G.queries;
+      const int qrow = live ? (b + qi / P.group) * P.hq + h * P.group + qi % P.group : 0;
+      const unsigned char* qp = static_cast<const unsigned char*>(P.q) + (size_t)qrow * kRowBytes;
+      if (kDense) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qb[nq][kk][0] = live ? *reinterpret_cast<const uint32_t*>(qp + 32 * kk + 4 * t) : 0u;
+          qb[nq][kk][1] = live ? *reinterpret_cast<const uint32_t*>(qp + 32 * kk + 16 + 4 * t) : 0u;
+        }
+        fac[nq][0] = fac[nq][1] = P.scale_log2e;
+      } else {
+        // the row is brought to a magnitude of 1 by a power of two, so that fp16 holds a bf16 row too
+        float x[8][4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          // dims of step kk: 8 bits: bytes (0,2) and (1,3) of word kk of my 32; 4 bits: of group
+          // kk / 2 the nibbles (0,4), (1,5) or (2,6), (3,7) of my word
+          const int base = FMT == kCacheInt4 ? 32 * (kk >> 1) + 8 * t + 2 * (kk & 1) : 32 * t + 4 * kk;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = base + (FMT == kCacheInt4 ? (i & 1) * 4 + (i >> 1) : (i & 1) * 2 + (i >> 1));
+            float f = 0.f;
+            if (live) {
+              const uint16_t u = *reinterpret_cast<const uint16_t*>(qp + 2 * d);
+              f = BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+            }
+            x[kk][i] = f;
+            top = max(top, __float_as_uint(f) & 0x7f800000u);
+          }
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // zeros and rows with an infinity or a NaN stay as they are
+        if (top == 0u || top == 0x7f800000u) top = 0x3f800000u;
+        top = min(top, 0x7e800000u);
+        const float down = __uint_as_float(0x7f000000u - top);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qb[nq][kk][0] = pack_pair<false>(x[kk][0] * down, x[kk][1] * down);
+          qb[nq][kk][1] = pack_pair<false>(x[kk][2] * down, x[kk][3] * down);
+        }
+        const float up = __uint_as_float(top) * P.scale_log2e * (FMT == kCacheFp8 ? 256.f : 1.f);
+        fac[nq][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+        fac[nq][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+      }
+    }
+    float o[NQ][8][4];
+    float m_ref[NQ][2], l_run[NQ][2];
+    float c_ref = 1.1754944e-38f;       // power of two that V scales are taken relative to
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[nq][i][0] = o[nq][i][1] = o[nq][i][2] = o[nq][i][3] = 0.f;
+      m_ref[nq][0] = m_ref[nq][1] = -INFINITY;
+      l_run[nq][0] = l_run[nq][1] = 0.f;
+    }
+
+    bool more = true;
+    while (more) {
+      const int s = n % S;
+      const int tok0 = cur.tile * kAttendTile + r0;     // my 16 tokens
+      const int len = cur.len;
+      float ks[2][kNS], vs[2][kNS];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kNS; ++j) {
+          ks[i][j] = ks_next[i][j];
+          vs[i][j] = vs_next[i][j];
+        }
+      advance(nxt);
+      if (!kDense && n + 1 < my_tiles) fetch_scales(nxt);
+      if (!mbar_wait(&ctrl->full[s], (unsigned)((n / S) & 1), &ctrl->timeout)) {
+        if (lane == 0) atomicOr(P.status, kStatusTimeout);
+      }
+      if (tok0 < len) {
+        const uint32_t kbase = stage0 + (uint32_t)s * kStage, vbase = kbase + kKBytes;
+        const bool tail = tok0 + 16 > len;
+        // ---- S^T = K Q^T
+        float x[NQ][4];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) x[nq][0] = x[nq][1] = x[nq][2] = x[nq][3] = 0.f;
+        if (kDense) {
+          const int tk = r0 + (mi & 1) * 8 + lr;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const int c8 = 2 * kk + (mi >> 1);
+            uint32_t a[4];
+            ldmatrix_x4(a, kbase + (c8 >> 3) * kHalf + tk * 128 + (((c8 & 7) ^ (tk & 7)) << 4));
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) mma_any<kPBf16>(x[nq], a, qb[nq][kk][0], qb[nq][kk][1]);
+          }
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[nq][i] *= P.scale_log2e;
+        } else if (FMT == kCacheInt4) {
+          const int ta = r0 + g, tb = ta + 8;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t wa = lds32(kbase + ta * 64 + ((j ^ ((ta >> 1) & 3)) << 4) + 4 * t);
+            const uint32_t wb = lds32(kbase + tb * 64 + ((j ^ ((tb >> 1) & 3)) << 4) + 4 * t);
+            float part[NQ][4];
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) part[nq][0] = part[nq][1] = part[nq][2] = part[nq][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a[4] = {nibbles_of(wa, 2 * i), nibbles_of(wb, 2 * i), nibbles_of(wa, 2 * i + 1),
+                                     nibbles_of(wb, 2 * i + 1)};
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) mma_16816(part[nq], a, qb[nq][2 * j + i][0], qb[nq][2 * j + i][1]);
+            }
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[nq][i] += part[nq][i] * ks[i >> 1][j < kNS ? j : 0];
+          }
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[nq][i] *= fac[nq][i & 1];
+        } else {
+          const int ta = r0 + g, tb = ta + 8;
+          float y[NQ][4];
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) y[nq][0] = y[nq][1] = y[nq][2] = y[nq][3] = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 ua = lds128(kbase + ta * 128 + (((2 * t + half) ^ (ta & 7)) << 4));
+            const uint4 ub = lds128(kbase + tb * 128 + (((2 * t + half) ^ (tb & 7)) << 4));
+            const uint32_t wa[4] = {ua.x, ua.y, ua.z, ua.w}, wb[4] = {ub.x, ub.y, ub.z, ub.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a[4];
+              codes_of<FMT>(wa[i], a[0], a[2]);
+              codes_of<FMT>(wb[i], a[1], a[3]);
+              const int kk = 4 * half + i;
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+                mma_16816(half ? y[nq] : x[nq], a, qb[nq][kk][0], qb[nq][kk][1]);
+            }
+          }
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[nq][i] = (x[nq][i] + y[nq][i]) * (ks[i >> 1][0] * fac[nq][i & 1]);
+        }
+        if (tail) {
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tok0 + g + 8 * (i >> 1) >= len) x[nq][i] = -INFINITY;
+        }
+        // ---- the running maximum less the lift; a score has to exceed it by 2^4 to move it
+        bool rise = false;
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            rise |= fmaxf(x[nq][i], x[nq][i + 2]) > m_ref[nq][i] + (kLazyLog2 + kLiftLog2);
+        float c_new = c_ref;
+        if (!kDense) {
+          float vm = 0.f;
+#pragma unroll
+          for (int j = 0; j < kNS; ++j) vm = fmaxf(vm, fmaxf(fabsf(vs[0][j]), fabsf(vs[1][j])));
+          if (vm >= 2.f * c_ref) {
+            c_new = __uint_as_float(min(__float_as_uint(vm) & 0x7f800000u, 0x7e800000u));
+            rise = true;
+          }
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+          float back = 1.f;
+          if (!kDense) {
+#pragma unroll
+            for (int i = 16; i; i >>= 1) c_new = fmaxf(c_new, __shfl_xor_sync(0xffffffffu, c_new, i));
+            back = c_ref / c_new;
+            c_ref = c_new;
+          }
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float mx = fmaxf(x[nq][i], x[nq][i + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float m_new = fmaxf(m_ref[nq][i], mx - kLiftLog2);
+              const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref[nq][i] - m_new);
+              m_ref[nq][i] = m_new;
+              l_run[nq][i] *= alpha;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                o[nq][j][i] *= alpha * back;
+                o[nq][j][i + 2] *= alpha * back;
+              }
+            }
+        }
+        // ---- weights, scaled by V's scales, as B fragments (tokens along k)
+        uint32_t pb[NQ][kNS][2];
+        const float down = kDense ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(c_ref));
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[nq][i] - (m_ref[nq][i & 1] == -INFINITY ? 0.f : m_ref[nq][i & 1]));
+          l_run[nq][0] += p[0] + p[2];
+          l_run[nq][1] += p[1] + p[3];
+#pragma unroll
+          for (int j = 0; j < kNS; ++j) {
+            const float f0 = kDense ? 1.f : vs[0][j] * down, f1 = kDense ? 1.f : vs[1][j] * down;
+            pb[nq][j][0] = movmatrix_trans(pack_pair<kPBf16>(p[0] * f0, p[1] * f0));
+            pb[nq][j][1] = movmatrix_trans(pack_pair<kPBf16>(p[2] * f1, p[3] * f1));
+          }
+        }
+        // ---- O^T += V^T P^T
+        if (kDense) {
+          const int tv = r0 + (mi >> 1) * 8 + lr;
+          // values behind the length may be anything; a weight of zero does not hide a NaN
+          const int left = len - tok0;
+          const uint32_t k0 = !tail ? 0xffffffffu : (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
+          const uint32_t k1 = !tail ? 0xffffffffu : (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            const int c8 = 2 * mt + (mi & 1);
+            uint32_t a[4];
+            ldmatrix_x4_trans(a, vbase + (c8 >> 3) * kHalf + tv * 128 + (((c8 & 7) ^ (tv & 7)) << 4));
+            if (tail) {
+              a[0] &= k0; a[1] &= k0; a[2] &= k1; a[3] &= k1;
+            }
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) mma_any<kPBf16>(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
+          }
+        } else if (FMT == kCacheInt4) {
+          // lane g: dims 32 j + 4 g .. + 3 of group j, two bytes of a token
+          const int ta = r0 + 2 * t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int tk = ta + 8 * i;    // even: tk and tk + 1 have the same swizzle
+              const uint32_t at = vbase + tk * 64 + ((j ^ ((tk >> 1) & 3)) << 4) + 2 * g;
+              w[i] = lds16(at) | (lds16(at + 64) << 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a[4] = {nibbles_of(w[0], 2 * i), nibbles_of(w[0], 2 * i + 1), nibbles_of(w[1], 2 * i),
+                                     nibbles_of(w[1], 2 * i + 1)};
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+                mma_16816(o[nq][2 * j + i], a, pb[nq][j < kNS ? j : 0][0], pb[nq][j < kNS ? j : 0][1]);
+            }
+          }
+        } else {
+          // lane g: dims 16 g .. 16 g + 15; tile mt takes bytes 2 mt and 2 mt + 1
+          const int ta = r0 + 2 * t;
+          uint4 u[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tk = ta + (i & 1) + 8 * (i >> 1);
+            u[i] = lds128(vbase + tk * 128 + ((g ^ (tk & 7)) << 4));
+          }
+          const uint32_t w[4][4] = {{u[0].x, u[0].y, u[0].z, u[0].w}, {u[1].x, u[1].y, u[1].z, u[1].w},
+                                    {u[2].x, u[2].y, u[2].z, u[2].w}, {u[3].x, u[3].y, u[3].z, u[3].w}};
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            const uint32_t sel = (mt & 1) ? 0x7632u : 0x5410u;
+            uint32_t a[4];
+            codes_of<FMT>(__byte_perm(w[0][mt >> 1], w[1][mt >> 1], sel), a[0], a[1]);
+            codes_of<FMT>(__byte_perm(w[2][mt >> 1], w[3][mt >> 1], sel), a[2], a[3]);
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) mma_16816(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->empty[s]);
+      ++n;
+      const int inner = cur.inner, bb = cur.b;
+      advance(cur);
+      more = n < my_tiles && cur.inner == inner && cur.b == bb;
+    }
+
+    // ---- merge the warps' partials and leave them in the row's slot
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float l = l_run[nq][i];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (g == 0) {
+          ctrl->m[warp][8 * nq + 2 * t + i] = m_ref[nq][i];
+          ctrl->l[warp][8 * nq + 2 * t + i] = l;
+        }
+      }
+    attend_consumer_sync();
+    const long long slot = row + blockIdx.x;
+    if (tid < QT) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, ctrl->m[w][tid]);
+#pragma unroll
+      for (int w = 0; w < kAttendWarps; ++w) {
+        // a warp without a maximum has l = 0, or a NaN that has to show
+        l += ctrl->m[w][tid] == -INFINITY ? ctrl->l[w][tid] : ctrl->l[w][tid] * fast_exp2(ctrl->m[w][tid] - m);
+      }
+      float* ml = G.part_ml + (slot * QT + tid) * 2;
+      ml[0] = m;
+      ml[1] = l;
+    }
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int qi = 8 * nq + 2 * t + i;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, ctrl->m[w][qi]);
+        f[i] = m_ref[nq][i] == -INFINITY ? 1.f : fast_exp2(m_ref[nq][i] - m);
+        if (!kDense) f[i] *= c_ref * (FMT == kCacheFp8 ? 256.f : 1.f);
+      }
+      // dims of the accumulators: 16-bit: 16 mt + g (+ 8); 8 bits: 16 g + 2 mt (+ 1); 4 bits: of group
+      // mt / 2: 4 g + 2 (mt & 1) (+ 1).  One half of the dims after the other through the buffer.
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (nq || half) attend_consumer_sync();
+        float* dst = sm_o + (warp * 8) * kMergePitch;
+        if (FMT == kCacheInt8 || FMT == kCacheFp8) {
+          if ((g >> 2) == half) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int mt = 0; mt < 8; ++mt)
+                *reinterpret_cast<float2*>(dst + (2 * t + i) * kMergePitch + 16 * (g & 3) + 2 * mt) =
+                    make_float2(o[nq][mt][i] * f[i], o[nq][mt][i + 2] * f[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int m4 = 0; m4 < 4; ++m4) {
+              const int mt = 4 * half + m4;
+              float* p = dst + (2 * t + i) * kMergePitch;
+              if (FMT == kCacheInt4) {
+                *reinterpret_cast<float2*>(p + 32 * (m4 >> 1) + 4 * g + 2 * (m4 & 1)) =
+                    make_float2(o[nq][mt][i] * f[i], o[nq][mt][i + 2] * f[i]);
+              } else {
+                p[16 * m4 + g] = o[nq][mt][i] * f[i];
+                p[16 * m4 + g + 8] = o[nq][mt][i + 2] * f[i];
+              }
+            }
+        }
+        attend_consumer_sync();
+        // 8 queries x 64 dims: 128 threads, one float4 each
+        const int qi = tid >> 4, d4 = tid & 15;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * 8 + qi) * kMergePitch + 4 * d4);
+          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        *reinterpret_cast<float4*>(G.part_o + ((slot * QT + 8 * nq + qi) * kHeadDim + 64 * half + 4 * d4)) = sum;
+      }
+    }
+    attend_consumer_sync();   // the buffers are reused by the next row
+  }
+}
+
+// Joins the partials of both segments for 8 (row, head) pairs, a warp each: weights by the common
+// maximum, sums in slot order (the same bits every time), zeros where nothing was seen.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+cache_combine_kernel(const __grid_constant__ CombineParams P) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= (long long)P.batch * P.hq) return;
+  const int b = (int)(r / P.hq), hq = (int)(r % P.hq), h = hq / P.group;
+  float m = -INFINITY, w = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const CombineSegment& G = P.seg[i];
+    if (!G.part_o) continue;
+    const int cache = G.prefix ? 0 : b;
+    const int qi = hq % P.group + (G.prefix ? b * P.group : 0);
+    const int per_cache = P.hkv * G.query_tiles, inner = h * G.query_tiles + qi / G.qt;
+    const long long at = G.line[cache], tiles = G.line[cache + 1] - at;
+    if (tiles == 0) continue;
+    const long long total = G.line[G.prefix ? 1 : P.batch] * per_cache;
+    const long long x0 = at * per_cache + inner * tiles, x1 = x0 + tiles - 1;
+    const long long ctas = min((long long)G.grid, total);
+    const int c0 = (int)(((x0 + 1) * ctas - 1) / total), c1 = (int)(((x1 + 1) * ctas - 1) / total);
+    const long long slot0 = (long long)cache * per_cache + inner;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const long long e = (slot0 + c) * G.qt + qi % G.qt;
+      const float2 ml = *reinterpret_cast<const float2*>(G.part_ml + 2 * e);
+      const float4 v = *reinterpret_cast<const float4*>(G.part_o + e * kHeadDim + 4 * lane);
+      const float top = fmaxf(m, ml.x), use = top == -INFINITY ? 0.f : top;
+      const float keep = fast_exp2(m - use);
+      // a partial without a maximum holds zeros, or a NaN that has to show
+      const float f = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - use);
+      m = top;
+      w = w * keep + ml.y * f;
+      sum.x = sum.x * keep + v.x * f;
+      sum.y = sum.y * keep + v.y * f;
+      sum.z = sum.z * keep + v.z * f;
+      sum.w = sum.w * keep + v.w * f;
+    }
+  }
+  // m = -inf with keep = 0 drops nothing: nothing finite was there
+  const float inv = w == 0.f ? 0.f : 1.f / w;
+  const uint2 u = make_uint2(pack_pair<BF16>(sum.x * inv, sum.y * inv), pack_pair<BF16>(sum.z * inv, sum.w * inv));
+  *reinterpret_cast<uint2*>(static_cast<unsigned char*>(P.out) + (size_t)r * kRowBytes + 8 * lane) = u;
+}
+
+namespace {
+int stage_bytes(int format) { return 2 * kAttendTile * cache_row_bytes(format); }
+}  // namespace
+
+// Three CTAs of a multiprocessor share 228 KiB, or two.
+int cache_attend_stages(int format, int nq) {
+  const int n = (nq == 1 ? 65536 : 98304) / stage_bytes(format);
+  return n < kAttendMaxStages ? n : kAttendMaxStages;
 }
 
 namespace {
 
-template <int FMT>
-cudaError_t launch_one(const CacheAttendParams& P, bool bf16, cudaStream_t stream) {
-  const dim3 grid(P.splits, P.batch * P.hq);
+template <int FMT, bool BF16, int NQ>
+cudaError_t launch_one(const CacheAttendParams& P, cudaStream_t stream) {
+  auto kern = cache_attend_kernel<FMT, BF16, NQ>;
+  const size_t smem = (size_t)P.seg.nstages * stage_bytes(FMT) + kMergeBytes + sizeof(AttendCtrl<NQ>) + 1024;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   note_launch();
-  if (bf16) cache_attend_kernel<FMT, true><<<grid, 32 * kAttendWarps, 0, stream>>>(P);
-  else cache_attend_kernel<FMT, false><<<grid, 32 * kAttendWarps, 0, stream>>>(P);
+  kern<<<P.seg.grid, kAttendThreads, smem, stream>>>(P);
   return cudaGetLastError();
+}
+
+template <int FMT>
+cudaError_t launch_format(const CacheAttendParams& P, bool bf16, int nq, cudaStream_t stream) {
+  if (bf16) return nq == 1 ? launch_one<FMT, true, 1>(P, stream) : launch_one<FMT, true, 2>(P, stream);
+  return nq == 1 ? launch_one<FMT, false, 1>(P, stream) : launch_one<FMT, false, 2>(P, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_cache_attend(const CacheAttendParams& P, int format, bool bf16, cudaStream_t stream) {
+cudaError_t launch_cache_attend(const CacheAttendParams& P, int format, bool bf16, int nq, cudaStream_t stream) {
   switch (format) {
-    case kCacheFp16: return launch_one<kCacheFp16>(P, bf16, stream);
-    case kCacheBf16: return launch_one<kCacheBf16>(P, bf16, stream);
-    case kCacheInt8: return launch_one<kCacheInt8>(P, bf16, stream);
-    case kCacheFp8: return launch_one<kCacheFp8>(P, bf16, stream);
-    default: return launch_one<kCacheInt4>(P, bf16, stream);
+    case kCacheFp16:
+      return nq == 1 ? launch_one<kCacheFp16, false, 1>(P, stream) : launch_one<kCacheFp16, false, 2>(P, stream);
+    case kCacheBf16:
+      return nq == 1 ? launch_one<kCacheBf16, true, 1>(P, stream) : launch_one<kCacheBf16, true, 2>(P, stream);
+    case kCacheInt8: return launch_format<kCacheInt8>(P, bf16, nq, stream);
+    case kCacheFp8: return launch_format<kCacheFp8>(P, bf16, nq, stream);
+    default: return launch_format<kCacheInt4>(P, bf16, nq, stream);
   }
 }
 
-cudaError_t launch_cache_combine(const float* a, int na, const float* b, int nb, int rows, void* out, bool bf16,
-                                 cudaStream_t stream) {
+cudaError_t launch_cache_combine(const CombineParams& P, bool bf16, cudaStream_t stream) {
+  // launched while the attention kernel before it still runs; it waits for that kernel's end itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((long long)P.batch * P.hq + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   note_launch();
-  if (bf16) cache_combine_kernel<true><<<rows, kHeadDim, 0, stream>>>(a, na, b, nb, out);
-  else cache_combine_kernel<false><<<rows, kHeadDim, 0, stream>>>(a, na, b, nb, out);
-  return cudaGetLastError();
+  return bf16 ? cudaLaunchKernelEx(&cfg, cache_combine_kernel<true>, P)
+              : cudaLaunchKernelEx(&cfg, cache_combine_kernel<false>, P);
 }
 
 }  // namespace ra
