@@ -106,7 +106,11 @@ int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int forma
   const CUresult r = enc(map, type, 4, const_cast<void*>(base), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE,
                          format == RA_CACHE_INT4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         // no more than the row: what lies behind it is another head's
+                         dense                       ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                         : format == RA_CACHE_INT4 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
+                                                   : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return RA_OK;
   char buf[96];
   snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -116,7 +120,7 @@ int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int forma
 // How one segment is worked on, and where its partials lie in the scratch.
 struct SegmentPlan {
   int caches, queries, nq, query_tiles, grid;
-  size_t ml_at, line_at, bytes;   // part_o at 0
+  size_t ml_at, span_at, bytes;   // part_o at 0
 };
 
 constexpr int kMaxSms = 256;      // bound of the device-independent workspace size
@@ -131,13 +135,13 @@ SegmentPlan plan_segment(bool prefix, int batch, int hq, int hkv, int tokens, in
   s.nq = s.queries <= 8 ? 1 : 2;
   s.query_tiles = (s.queries + 8 * s.nq - 1) / (8 * s.nq);
   const long long rows = (long long)s.caches * hkv * s.query_tiles;
-  const long long tiles = rows * ((tokens + kAttendTile - 1) / kAttendTile);
-  s.grid = (int)std::min<long long>(tiles, (long long)attend_ctas(s.nq) * sms);
+  const long long units = rows * ((tokens + kAttendTile - 1) / kAttendTile + kAttendRowUnits);
+  s.grid = (int)std::min<long long>(units, (long long)attend_ctas(s.nq) * sms);
   const size_t slots = (size_t)rows + s.grid;
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   s.ml_at = up(slots * 8 * s.nq * kHeadDim * sizeof(float));
-  s.line_at = s.ml_at + up(slots * 8 * s.nq * 2 * sizeof(float));
-  s.bytes = s.line_at + up((size_t)(s.caches + 1) * sizeof(long long));
+  s.span_at = s.ml_at + up(slots * 8 * s.nq * 2 * sizeof(float));
+  s.bytes = s.span_at + up((size_t)rows * 2 * sizeof(int));
   return s;
 }
 
@@ -233,17 +237,19 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
     g.nstages = cache_attend_stages(format, s.nq);
     g.part_o = reinterpret_cast<float*>(at);
     g.part_ml = reinterpret_cast<float*>(at + s.ml_at);
-    g.line = reinterpret_cast<long long*>(at + s.line_at);
+    g.span = reinterpret_cast<int*>(at + s.span_at);
     a.q = p->q;
     a.status = static_cast<unsigned*>(p->status);
     a.hq = p->num_q_heads;
     a.hkv = p->num_kv_heads;
     a.group = cp.group;
+    a.after = i == 1 && has[0];
     a.scale_log2e = p->sm_scale * kLog2e;
     CombineSegment& c = cp.seg[i];
     c.part_o = g.part_o;
     c.part_ml = g.part_ml;
-    c.line = g.line;
+    c.span = g.span;
+    c.lens = g.lens;
     c.queries = s.queries;
     c.query_tiles = s.query_tiles;
     c.qt = 8 * s.nq;

@@ -81,19 +81,19 @@ __device__ __forceinline__ uint32_t hsub2_bits(uint32_t a, uint32_t b) {
   return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// Two pairs of fp16 codes out of the bytes (0,2) and (1,3) of a word.  int8: a byte with its sign bit
-// flipped, put into the low mantissa bits of 1024.0, is 1024 + 128 + code.  e4m3: sign and the
-// seven other bits moved to fp16's places give code * 2^-8 (the exponents' biases differ by 8),
-// subnormals included.
+// Two pairs of fp16 codes out of the four bytes of a word, (0,2) and (1,3) for int8: a byte with its
+// sign bit flipped, put into the low mantissa bits of 1024.0, is 1024 + 128 + code.  e4m3: (0,1) and
+// (2,3) by the hardware's conversion.
 template <int FMT>
-__device__ __forceinline__ void codes_of(uint32_t w, uint32_t& even, uint32_t& odd) {
+__device__ __forceinline__ void codes_of(uint32_t w, uint32_t& first, uint32_t& second) {
   if (FMT == kCacheInt8) {
-    even = hsub2_bits((w & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
-    odd = hsub2_bits(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+    first = hsub2_bits((w & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+    second = hsub2_bits(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
   } else {
-    const uint32_t x = w << 8;
-    even = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
-    odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(first), "=r"(second)
+        : "r"(w));
   }
 }
 // nibbles (i, i + 4) of a word, which hold code + 8
@@ -101,10 +101,13 @@ __device__ __forceinline__ uint32_t nibbles_of(uint32_t w, int i) {
   return hsub2_bits(((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, 0x64086408u);
 }
 
-// The place in the line of work rows: cache, (kv head, query tile), tile of tokens.
-struct AttendWalk {
-  int b, inner, tile, len, tiles;
+// My part of one work row: tiles [first, first + count) of (cache b, kv head h, query tile qt), and the
+// units of the line that it stands for.
+struct AttendRow {
+  int b, inner, h, qt, len, first, count, units;
 };
+
+constexpr float kNoMax = -3e38f;    // below every score that counts, and finite: no special cases
 
 template <int FMT, bool BF16, int NQ>
 __global__ void __launch_bounds__(kAttendThreads, attend_ctas(NQ))
@@ -140,17 +143,25 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     if (G.lens) len = max(0, min(len, G.lens[b]));
     return len;
   };
-  auto tiles_of = [&](int b) { return ceil_div(length_of(b), kAttendTile); };
+  auto units_of_length = [](int len) { return len > 0 ? ceil_div(len, kAttendTile) + kAttendRowUnits : 0; };
+  auto units_of = [&](int b) { return units_of_length(length_of(b)); };
 
-  // ---- my share of the line: every thread sums a run of caches, a block-wide scan does the rest
-  {
+  // ---- my share of the line.  Equal lengths need a division; otherwise every thread sums a run of
+  // caches and a block-wide scan does the rest.
+  if (!G.lens) {
+    const long long n = units_of(0), all = n * G.caches * per_cache, ctas = min((long long)G.grid, all);
+    if (tid == 0) {
+      ctrl->total = n * G.caches;
+      ctrl->start = blockIdx.x < ctas ? (int)(all * blockIdx.x / ctas / (n * per_cache)) : 0;
+      ctrl->before = ctrl->start * n;
+    }
+  } else {
     const int run = ceil_div(G.caches, kAttendThreads);
     const int lo = min(G.caches, tid * run), hi = min(G.caches, lo + run);
     long long mine = 0;
     for (int b = lo; b < hi; ++b) {
-      mine += tiles_of(b);
-      if (G.lens && blockIdx.x == 0 && (G.lens[b] < 0 || G.lens[b] > G.cache.n_tokens))
-        atomicOr(P.status, kStatusBadToken);
+      mine += units_of(b);
+      if (blockIdx.x == 0 && (G.lens[b] < 0 || G.lens[b] > G.cache.n_tokens)) atomicOr(P.status, kStatusBadToken);
     }
     long long incl = mine;
 #pragma unroll
@@ -166,74 +177,93 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
       if (w < warp) base += ctrl->sums[w];
       total += ctrl->sums[w];
     }
-    long long at = base + incl - mine;          // tiles of one (kv head, query tile) before cache lo
+    long long at = base + incl - mine;          // units of one (kv head, query tile) before cache lo
     const long long all = total * per_cache;
-    const long long ctas = min((long long)G.grid, all);   // every one of them has a tile
+    const long long ctas = min((long long)G.grid, all);   // every one of them has a unit
     const long long first = blockIdx.x < ctas ? all * blockIdx.x / ctas : all;
     for (int b = lo; b < hi; ++b) {
-      const int n = tiles_of(b);
-      if (blockIdx.x == 0) G.line[b] = at;
+      const int n = units_of(b);
       if (first >= at * per_cache && first < (at + n) * per_cache) {
         ctrl->start = b;
         ctrl->before = at;
       }
       at += n;
     }
-    if (tid == 0) {
-      ctrl->total = total;
-      if (blockIdx.x == 0) G.line[G.caches] = total;
-    }
-    __syncthreads();
+    if (tid == 0) ctrl->total = total;
   }
-  // lets the combine kernel start its launch; it waits for this grid's end before it reads
+  __syncthreads();
+  // lets the next kernel start its launch; it waits for this grid's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long total = ctrl->total * per_cache;
   const long long ctas = min((long long)G.grid, total);
-  if (blockIdx.x >= ctas) return;
-  const long long t0 = total * blockIdx.x / ctas, t1 = total * (blockIdx.x + 1) / ctas;
-  const int my_tiles = (int)(t1 - t0);
-
-  AttendWalk cur;
-  {
-    cur.b = ctrl->start;
-    cur.len = length_of(cur.b);
-    cur.tiles = ceil_div(cur.len, kAttendTile);
-    const int off = (int)(t0 - ctrl->before * per_cache);
-    cur.inner = off / cur.tiles;
-    cur.tile = off % cur.tiles;
+  if (blockIdx.x >= ctas) {
+    if (P.after) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
   }
-  auto advance = [&](AttendWalk& w) {
-    if (++w.tile < w.tiles) return;
-    w.tile = 0;
-    if (++w.inner < per_cache) return;
-    w.inner = 0;
-    do {
-      ++w.b;
-      w.len = w.b < G.caches ? length_of(w.b) : 1;
-      w.tiles = ceil_div(w.len, kAttendTile);
-    } while (w.tiles == 0);
+  const long long t0 = total * blockIdx.x / ctas, t1 = total * (blockIdx.x + 1) / ctas;
+  int left = (int)(t1 - t0);          // units of mine in this row and behind it
+
+  // r's units from `pos` on, of which n are mine or behind
+  auto take = [&](AttendRow& r, int pos, int n) {
+    r.units = min(n, units_of_length(r.len) - pos);
+    r.first = max(0, pos - kAttendRowUnits);
+    r.count = max(0, pos + r.units - kAttendRowUnits - r.first);
+  };
+  AttendRow row;
+  {
+    row.b = ctrl->start;
+    row.len = length_of(row.b);
+    const int units = units_of_length(row.len);
+    const long long off = t0 - ctrl->before * per_cache;
+    row.inner = (int)(off / units);
+    row.h = row.inner / G.query_tiles;
+    row.qt = row.inner % G.query_tiles;
+    take(row, (int)(off % units), left);
+  }
+  // the row behind `r`, of which n > 0 units are mine or behind
+  auto row_behind = [&](AttendRow r, int n) {
+    ++r.inner;
+    if (++r.qt == G.query_tiles) {
+      r.qt = 0;
+      ++r.h;
+    }
+    if (r.inner == per_cache) {
+      r.inner = r.h = r.qt = 0;
+      do r.len = length_of(++r.b);
+      while (r.len == 0);
+    }
+    take(r, 0, n);
+    return r;
   };
 
   if (warp == kAttendWarps) {
     // ---------------------------------------------------------------- producer warp
     if (lane == 0) {
-      for (int n = 0; n < my_tiles; ++n) {
-        const int s = n % S;
-        if (n >= S && !mbar_wait(&ctrl->empty[s], (unsigned)(((n / S) - 1) & 1), &ctrl->timeout))
-          atomicOr(P.status, kStatusTimeout);
-        unsigned char* dst = smem + (size_t)s * kStage;
-        const int tok = cur.tile * kAttendTile, h = cur.inner / G.query_tiles;
-        mbar_expect_tx(&ctrl->full[s], kStage);
-        if (kDense) {
-          tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, h, tok, cur.b);
-          tma_load_4d(dst + kHalf, &G.kmap, &ctrl->full[s], 64, h, tok, cur.b);
-          tma_load_4d(dst + 2 * kHalf, &G.vmap, &ctrl->full[s], 0, h, tok, cur.b);
-          tma_load_4d(dst + 3 * kHalf, &G.vmap, &ctrl->full[s], 64, h, tok, cur.b);
-        } else {
-          tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, h, tok, cur.b);
-          tma_load_4d(dst + kKBytes, &G.vmap, &ctrl->full[s], 0, h, tok, cur.b);
+      int s = 0;
+      unsigned parity = 1;          // of the phase before the first: an unused stage is free
+      for (;;) {
+        for (int i = 0; i < row.count; ++i) {
+          if (!mbar_wait(&ctrl->empty[s], parity, &ctrl->timeout)) atomicOr(P.status, kStatusTimeout);
+          unsigned char* dst = smem + (size_t)s * kStage;
+          const int tok = (row.first + i) * kAttendTile;
+          mbar_expect_tx(&ctrl->full[s], kStage);
+          if (kDense) {
+            tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, row.h, tok, row.b);
+            tma_load_4d(dst + kHalf, &G.kmap, &ctrl->full[s], 64, row.h, tok, row.b);
+            tma_load_4d(dst + 2 * kHalf, &G.vmap, &ctrl->full[s], 0, row.h, tok, row.b);
+            tma_load_4d(dst + 3 * kHalf, &G.vmap, &ctrl->full[s], 64, row.h, tok, row.b);
+          } else {
+            tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, row.h, tok, row.b);
+            tma_load_4d(dst + kKBytes, &G.vmap, &ctrl->full[s], 0, row.h, tok, row.b);
+          }
+          if (++s == S) {
+            s = 0;
+            parity ^= 1;
+          }
         }
-        advance(cur);
+        left -= row.units;
+        if (left <= 0) break;
+        row = row_behind(row, left);
       }
     }
     return;
@@ -247,36 +277,57 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
   // scales of the next tile, fetched one tile ahead: tokens g and g + 8 of my 16
   constexpr int kNS = kDense ? 1 : cache_row_scales(FMT);
   float ks_next[2][kNS], vs_next[2][kNS];
-  auto fetch_scales = [&](const AttendWalk& w) {
-    if (kDense) return;
-    const int h = w.inner / G.query_tiles;
-    const long long base = (long long)w.b * G.cache.sbstride + (long long)h * G.cache.shstride;
+  auto fetch_scales = [&](const float* kp, const float* vp, int tok, int len) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int tok = w.tile * kAttendTile + r0 + g + 8 * i;
-      const bool live = tok < w.len;
-      const float* kp = G.cache.k_scale + base + (long long)tok * kNS;
-      const float* vp = G.cache.v_scale + base + (long long)tok * kNS;
+      const bool live = tok + 8 * i < len;
       if (kNS == 4) {
         const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = live ? __ldg(reinterpret_cast<const float4*>(kp)) : z;
-        const float4 b = live ? __ldg(reinterpret_cast<const float4*>(vp)) : z;
+        const float4 a = live ? __ldg(reinterpret_cast<const float4*>(kp) + 8 * i) : z;
+        const float4 b = live ? __ldg(reinterpret_cast<const float4*>(vp) + 8 * i) : z;
         ks_next[i][0] = a.x; ks_next[i][kNS > 1 ? 1 : 0] = a.y; ks_next[i][kNS > 2 ? 2 : 0] = a.z; ks_next[i][kNS - 1] = a.w;
         vs_next[i][0] = b.x; vs_next[i][kNS > 1 ? 1 : 0] = b.y; vs_next[i][kNS > 2 ? 2 : 0] = b.z; vs_next[i][kNS - 1] = b.w;
       } else {
-        ks_next[i][0] = live ? __ldg(kp) : 0.f;
-        vs_next[i][0] = live ? __ldg(vp) : 0.f;
+        ks_next[i][0] = live ? __ldg(kp + 8 * i) : 0.f;
+        vs_next[i][0] = live ? __ldg(vp + 8 * i) : 0.f;
       }
     }
   };
-  if (!kDense) fetch_scales(cur);
-  AttendWalk nxt = cur;
+  // where this lane's scales of a row's tile begin
+  auto scale_offset = [&](const AttendRow& r, int tile) {
+    return (long long)r.b * G.cache.sbstride + (long long)r.h * G.cache.shstride +
+           (long long)(tile * kAttendTile + r0 + g) * kNS;
+  };
+  if (!kDense) {
+    const long long at = scale_offset(row, row.first);
+    fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, row.first * kAttendTile + r0 + g, row.len);
+  }
 
-  int n = 0;
-  while (n < my_tiles) {
+  int s = 0;
+  unsigned parity = 0;
+  for (;;) {
     // ---- one work row
-    const int b = cur.b, h = cur.inner / G.query_tiles, q0 = (cur.inner % G.query_tiles) * QT;
-    const long long row = (long long)b * per_cache + cur.inner;
+    left -= row.units;
+    AttendRow behind = row;
+    if (left > 0) behind = row_behind(row, left);
+    if (row.count == 0) {             // none of its tiles, only of the units before them
+      if (left <= 0) break;
+      row = behind;
+      if (!kDense) {
+        const long long at = scale_offset(row, 0);
+        fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, r0 + g, row.len);
+      }
+      continue;
+    }
+    const int b = row.b, h = row.h, q0 = row.qt * QT, len = row.len;
+    const long long slot = (long long)b * per_cache + row.inner + blockIdx.x;
+    const float* kp = nullptr;
+    const float* vp = nullptr;
+    if (!kDense) {
+      const long long at = scale_offset(row, row.first);
+      kp = G.cache.k_scale + at;
+      vp = G.cache.v_scale + at;
+    }
     // B fragments of Q^T: column g is query q0 + 8 nq + g; the dims of lane t in the order K's lanes hold them
     uint32_t qb[NQ][8][2];
     float fac[NQ][2];      // what turns a raw score of my two columns into the log2 domain
@@ -284,6 +335,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     for (int nq = 0; nq < NQ; ++nq) {
       const int qi = q0 + 8 * nq + g;
       const bool live = qi < G.queries;
+      // of the prefix (one cache) query qi is of batch row qi / group
       const int qrow = live ? (b + qi / P.group) * P.hq + h * P.group + qi % P.group : 0;
       const unsigned char* qp = static_cast<const unsigned char*>(P.q) + (size_t)qrow * kRowBytes;
       if (kDense) {
@@ -295,25 +347,29 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         fac[nq][0] = fac[nq][1] = P.scale_log2e;
       } else {
         // the row is brought to a magnitude of 1 by a power of two, so that fp16 holds a bf16 row too
-        float x[8][4];
+        // dims of step kk: int8: bytes (0,2), (1,3) of word kk of my 32 dims; e4m3: bytes (0,1), (2,3);
+        // int4: of group kk / 2, nibbles (0,4), (1,5) or (2,6), (3,7) of my word
+        float x[32];
         uint32_t top = 0;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          // dims of step kk: 8 bits: bytes (0,2) and (1,3) of word kk of my 32; 4 bits: of group
-          // kk / 2 the nibbles (0,4), (1,5) or (2,6), (3,7) of my word
-          const int base = FMT == kCacheInt4 ? 32 * (kk >> 1) + 8 * t + 2 * (kk & 1) : 32 * t + 4 * kk;
+        for (int i = 0; i < 4; ++i) {
+          const uint4 u = live ? *reinterpret_cast<const uint4*>(qp + (FMT == kCacheInt4 ? 64 * i + 16 * t : 64 * t + 16 * i))
+                               : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = base + (FMT == kCacheInt4 ? (i & 1) * 4 + (i >> 1) : (i & 1) * 2 + (i >> 1));
-            float f = 0.f;
-            if (live) {
-              const uint16_t u = *reinterpret_cast<const uint16_t*>(qp + 2 * d);
-              f = BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+          for (int j = 0; j < 4; ++j) {
+            if (BF16) {
+              x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+              x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+              const float2 f = h2f2(w[j]);
+              x[8 * i + 2 * j] = f.x;
+              x[8 * i + 2 * j + 1] = f.y;
             }
-            x[kk][i] = f;
-            top = max(top, __float_as_uint(f) & 0x7f800000u);
           }
         }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7f800000u);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // zeros and rows with an infinity or a NaN stay as they are
@@ -322,10 +378,13 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         const float down = __uint_as_float(0x7f000000u - top);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          qb[nq][kk][0] = pack_pair<false>(x[kk][0] * down, x[kk][1] * down);
-          qb[nq][kk][1] = pack_pair<false>(x[kk][2] * down, x[kk][3] * down);
+          const float* y = FMT == kCacheInt4 ? x + 8 * (kk >> 1) + 2 * (kk & 1) : x + 4 * kk;
+          constexpr int i1 = FMT == kCacheInt4 ? 4 : FMT == kCacheInt8 ? 2 : 1;
+          constexpr int i2 = FMT == kCacheFp8 ? 2 : 1;
+          qb[nq][kk][0] = pack_pair<false>(y[0] * down, y[i1] * down);
+          qb[nq][kk][1] = pack_pair<false>(y[i2] * down, y[i2 + i1] * down);
         }
-        const float up = __uint_as_float(top) * P.scale_log2e * (FMT == kCacheFp8 ? 256.f : 1.f);
+        const float up = __uint_as_float(top) * P.scale_log2e;
         fac[nq][0] = __shfl_sync(0xffffffffu, up, 8 * t);
         fac[nq][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
       }
@@ -337,26 +396,31 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[nq][i][0] = o[nq][i][1] = o[nq][i][2] = o[nq][i][3] = 0.f;
-      m_ref[nq][0] = m_ref[nq][1] = -INFINITY;
+      m_ref[nq][0] = m_ref[nq][1] = kNoMax;
       l_run[nq][0] = l_run[nq][1] = 0.f;
     }
 
-    bool more = true;
-    while (more) {
-      const int s = n % S;
-      const int tok0 = cur.tile * kAttendTile + r0;     // my 16 tokens
-      const int len = cur.len;
+    for (int i_tile = 0; i_tile < row.count; ++i_tile) {
+      const int tok0 = (row.first + i_tile) * kAttendTile + r0;     // my 16 tokens
       float ks[2][kNS], vs[2][kNS];
+      if (!kDense) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < kNS; ++j) {
-          ks[i][j] = ks_next[i][j];
-          vs[i][j] = vs_next[i][j];
+          for (int j = 0; j < kNS; ++j) {
+            ks[i][j] = ks_next[i][j];
+            vs[i][j] = vs_next[i][j];
+          }
+        if (i_tile + 1 < row.count) {
+          kp += kAttendTile * kNS;
+          vp += kAttendTile * kNS;
+          fetch_scales(kp, vp, tok0 + kAttendTile + g, len);
+        } else if (left > 0) {
+          const long long at = scale_offset(behind, 0);
+          fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, r0 + g, behind.len);
         }
-      advance(nxt);
-      if (!kDense && n + 1 < my_tiles) fetch_scales(nxt);
-      if (!mbar_wait(&ctrl->full[s], (unsigned)((n / S) & 1), &ctrl->timeout)) {
+      }
+      if (!mbar_wait(&ctrl->full[s], parity, &ctrl->timeout)) {
         if (lane == 0) atomicOr(P.status, kStatusTimeout);
       }
       if (tok0 < len) {
@@ -472,7 +536,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
               const float m_new = fmaxf(m_ref[nq][i], mx - kLiftLog2);
-              const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref[nq][i] - m_new);
+              const float alpha = fast_exp2(m_ref[nq][i] - m_new);
               m_ref[nq][i] = m_new;
               l_run[nq][i] *= alpha;
 #pragma unroll
@@ -489,7 +553,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         for (int nq = 0; nq < NQ; ++nq) {
           float p[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[nq][i] - (m_ref[nq][i & 1] == -INFINITY ? 0.f : m_ref[nq][i & 1]));
+          for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[nq][i] - m_ref[nq][i & 1]);
           l_run[nq][0] += p[0] + p[2];
           l_run[nq][1] += p[1] + p[3];
 #pragma unroll
@@ -500,12 +564,13 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
           }
         }
         // ---- O^T += V^T P^T
+        // values behind the length may be anything, and a weight of zero does not hide an infinity or a
+        // NaN: they are cut out of the fragments (int8 and int4 codes are always finite)
+        const int seen = len - tok0;
+        const uint32_t k0 = !tail ? 0xffffffffu : (2 * t < seen ? 0xffffu : 0u) | (2 * t + 1 < seen ? 0xffff0000u : 0u);
+        const uint32_t k1 = !tail ? 0xffffffffu : (2 * t + 8 < seen ? 0xffffu : 0u) | (2 * t + 9 < seen ? 0xffff0000u : 0u);
         if (kDense) {
           const int tv = r0 + (mi >> 1) * 8 + lr;
-          // values behind the length may be anything; a weight of zero does not hide a NaN
-          const int left = len - tok0;
-          const uint32_t k0 = !tail ? 0xffffffffu : (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
-          const uint32_t k1 = !tail ? 0xffffffffu : (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) {
             const int c8 = 2 * mt + (mi & 1);
@@ -551,10 +616,14 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
                                     {u[2].x, u[2].y, u[2].z, u[2].w}, {u[3].x, u[3].y, u[3].z, u[3].w}};
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) {
-            const uint32_t sel = (mt & 1) ? 0x7632u : 0x5410u;
+            // bytes 2 mt and 2 mt + 1 of both tokens, paired as codes_of takes them
+            const uint32_t sel = FMT == kCacheInt8 ? ((mt & 1) ? 0x7632u : 0x5410u) : ((mt & 1) ? 0x7362u : 0x5140u);
             uint32_t a[4];
             codes_of<FMT>(__byte_perm(w[0][mt >> 1], w[1][mt >> 1], sel), a[0], a[1]);
             codes_of<FMT>(__byte_perm(w[2][mt >> 1], w[3][mt >> 1], sel), a[2], a[3]);
+            if (FMT == kCacheFp8 && tail) {
+              a[0] &= k0; a[1] &= k0; a[2] &= k1; a[3] &= k1;
+            }
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) mma_16816(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
           }
@@ -562,10 +631,10 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctrl->empty[s]);
-      ++n;
-      const int inner = cur.inner, bb = cur.b;
-      advance(cur);
-      more = n < my_tiles && cur.inner == inner && cur.b == bb;
+      if (++s == S) {
+        s = 0;
+        parity ^= 1;
+      }
     }
 
     // ---- merge the warps' partials and leave them in the row's slot
@@ -583,16 +652,18 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         }
       }
     attend_consumer_sync();
-    const long long slot = row + blockIdx.x;
+    if (tid == 0) {
+      // the first and the last CTA with tiles of this row say so
+      int* span = G.span + 2 * ((long long)b * per_cache + row.inner);
+      if (row.first == 0) span[0] = blockIdx.x;
+      if ((row.first + row.count) * kAttendTile >= len) span[1] = blockIdx.x;
+    }
     if (tid < QT) {
-      float m = -INFINITY, l = 0.f;
+      float m = kNoMax, l = 0.f;
 #pragma unroll
       for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, ctrl->m[w][tid]);
 #pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
-        // a warp without a maximum has l = 0, or a NaN that has to show
-        l += ctrl->m[w][tid] == -INFINITY ? ctrl->l[w][tid] : ctrl->l[w][tid] * fast_exp2(ctrl->m[w][tid] - m);
-      }
+      for (int w = 0; w < kAttendWarps; ++w) l += ctrl->l[w][tid] * fast_exp2(ctrl->m[w][tid] - m);
       float* ml = G.part_ml + (slot * QT + tid) * 2;
       ml[0] = m;
       ml[1] = l;
@@ -603,11 +674,11 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int qi = 8 * nq + 2 * t + i;
-        float m = -INFINITY;
+        float m = kNoMax;
 #pragma unroll
         for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, ctrl->m[w][qi]);
-        f[i] = m_ref[nq][i] == -INFINITY ? 1.f : fast_exp2(m_ref[nq][i] - m);
-        if (!kDense) f[i] *= c_ref * (FMT == kCacheFp8 ? 256.f : 1.f);
+        f[i] = fast_exp2(m_ref[nq][i] - m);
+        if (!kDense) f[i] *= c_ref;
       }
       // dims of the accumulators: 16-bit: 16 mt + g (+ 8); 8 bits: 16 g + 2 mt (+ 1); 4 bits: of group
       // mt / 2: 4 g + 2 (mt & 1) (+ 1).  One half of the dims after the other through the buffer.
@@ -652,21 +723,31 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         *reinterpret_cast<float4*>(G.part_o + ((slot * QT + 8 * nq + qi) * kHeadDim + 64 * half + 4 * d4)) = sum;
       }
     }
+    if (left <= 0) break;
+    row = behind;
     attend_consumer_sync();   // the buffers are reused by the next row
   }
+  // a kernel that waits for this one's end then has everything before it too
+  if (P.after) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the partials of both segments for 8 (row, head) pairs, a warp each: weights by the common
-// maximum, sums in slot order (the same bits every time), zeros where nothing was seen.
-template <bool BF16>
-__global__ void __launch_bounds__(256)
+// Joins the partials of both segments for one (row, head): weights by the common maximum, sums in
+// slot order (the same bits every time), zeros where nothing was seen.  A warp takes up to 32 partials
+// at once: a lane for the maximum and weight of each, then four dims per lane.  WARPS warps share the
+// partials of a row where rows are few, or each has a row of its own.
+constexpr int kCombineWarps = 8;
+
+template <bool BF16, int WARPS>
+__global__ void __launch_bounds__(32 * kCombineWarps)
 cache_combine_kernel(const __grid_constant__ CombineParams P) {
+  __shared__ float4 sm_sum[kCombineWarps][32];
+  __shared__ float2 sm_ml[kCombineWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * (kCombineWarps / WARPS) + warp / WARPS;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (r >= (long long)P.batch * P.hq) return;
   const int b = (int)(r / P.hq), hq = (int)(r % P.hq), h = hq / P.group;
-  float m = -INFINITY, w = 0.f;
+  float m = kNoMax, w = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -674,32 +755,51 @@ cache_combine_kernel(const __grid_constant__ CombineParams P) {
     if (!G.part_o) continue;
     const int cache = G.prefix ? 0 : b;
     const int qi = hq % P.group + (G.prefix ? b * P.group : 0);
-    const int per_cache = P.hkv * G.query_tiles, inner = h * G.query_tiles + qi / G.qt;
-    const long long at = G.line[cache], tiles = G.line[cache + 1] - at;
-    if (tiles == 0) continue;
-    const long long total = G.line[G.prefix ? 1 : P.batch] * per_cache;
-    const long long x0 = at * per_cache + inner * tiles, x1 = x0 + tiles - 1;
-    const long long ctas = min((long long)G.grid, total);
-    const int c0 = (int)(((x0 + 1) * ctas - 1) / total), c1 = (int)(((x1 + 1) * ctas - 1) / total);
-    const long long slot0 = (long long)cache * per_cache + inner;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const long long e = (slot0 + c) * G.qt + qi % G.qt;
-      const float2 ml = *reinterpret_cast<const float2*>(G.part_ml + 2 * e);
-      const float4 v = *reinterpret_cast<const float4*>(G.part_o + e * kHeadDim + 4 * lane);
-      const float top = fmaxf(m, ml.x), use = top == -INFINITY ? 0.f : top;
-      const float keep = fast_exp2(m - use);
-      // a partial without a maximum holds zeros, or a NaN that has to show
-      const float f = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - use);
+    const long long row = (long long)cache * P.hkv * G.query_tiles + h * G.query_tiles + qi / G.qt;
+    if (G.lens && G.lens[cache] <= 0) continue;
+    const int2 span = *reinterpret_cast<const int2*>(G.span + 2 * row);
+    const int c1 = span.y, per = min(32, (span.y - span.x + WARPS) / WARPS);
+    const long long e0 = row * G.qt + qi % G.qt;
+    for (int c = span.x + per * (warp % WARPS); c <= c1; c += per * WARPS) {
+      const int n = min(per, c1 - c + 1);
+      float2 ml = make_float2(kNoMax, 0.f);
+      if (lane < n) ml = *reinterpret_cast<const float2*>(G.part_ml + 2 * (e0 + (long long)(c + lane) * G.qt));
+      float top = fmaxf(m, ml.x);
+#pragma unroll
+      for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+      const float keep = fast_exp2(m - top), f = fast_exp2(ml.x - top);
       m = top;
-      w = w * keep + ml.y * f;
-      sum.x = sum.x * keep + v.x * f;
-      sum.y = sum.y * keep + v.y * f;
-      sum.z = sum.z * keep + v.z * f;
-      sum.w = sum.w * keep + v.w * f;
+      w = w * keep + ml.y * f;           // of this lane's partials; summed over the lanes at the end
+      sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+      const float* src = G.part_o + (e0 + (long long)c * G.qt) * kHeadDim + 4 * lane;
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(src + (long long)k * G.qt * kHeadDim);
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        sum.x += v.x * fk; sum.y += v.y * fk; sum.z += v.z * fk; sum.w += v.w * fk;
+      }
     }
   }
-  // m = -inf with keep = 0 drops nothing: nothing finite was there
+#pragma unroll
+  for (int k = 16; k; k >>= 1) w += __shfl_xor_sync(0xffffffffu, w, k);
+  if (WARPS > 1) {
+    sm_sum[warp][lane] = sum;
+    if (lane == 0) sm_ml[warp] = make_float2(m, w);
+    __syncthreads();
+    if (warp) return;
+    m = kNoMax;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) m = fmaxf(m, sm_ml[k].x);
+    w = 0.f;
+    sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float f = fast_exp2(sm_ml[k].x - m);
+      const float4 v = sm_sum[k][lane];
+      w += sm_ml[k].y * f;
+      sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
+    }
+  }
   const float inv = w == 0.f ? 0.f : 1.f / w;
   const uint2 u = make_uint2(pack_pair<BF16>(sum.x * inv, sum.y * inv), pack_pair<BF16>(sum.z * inv, sum.w * inv));
   *reinterpret_cast<uint2*>(static_cast<unsigned char*>(P.out) + (size_t)r * kRowBytes + 8 * lane) = u;
@@ -723,9 +823,18 @@ cudaError_t launch_one(const CacheAttendParams& P, cudaStream_t stream) {
   const size_t smem = (size_t)P.seg.nstages * stage_bytes(FMT) + kMergeBytes + sizeof(AttendCtrl<NQ>) + 1024;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)P.seg.grid);
+  cfg.blockDim = dim3(kAttendThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = P.after ? 1 : 0;
   note_launch();
-  kern<<<P.seg.grid, kAttendThreads, smem, stream>>>(P);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kern, P);
 }
 
 template <int FMT>
@@ -750,9 +859,11 @@ cudaError_t launch_cache_attend(const CacheAttendParams& P, int format, bool bf1
 
 cudaError_t launch_cache_combine(const CombineParams& P, bool bf16, cudaStream_t stream) {
   // launched while the attention kernel before it still runs; it waits for that kernel's end itself
+  const long long rows = (long long)P.batch * P.hq;
+  const bool share = rows <= 1024;      // up to about one wave of CTAs with all their warps on one row
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((long long)P.batch * P.hq + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)(share ? rows : (rows + kCombineWarps - 1) / kCombineWarps));
+  cfg.blockDim = dim3(32 * kCombineWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -760,8 +871,11 @@ cudaError_t launch_cache_combine(const CombineParams& P, bool bf16, cudaStream_t
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   note_launch();
-  return bf16 ? cudaLaunchKernelEx(&cfg, cache_combine_kernel<true>, P)
-              : cudaLaunchKernelEx(&cfg, cache_combine_kernel<false>, P);
+  if (share)
+    return bf16 ? cudaLaunchKernelEx(&cfg, cache_combine_kernel<true, kCombineWarps>, P)
+                : cudaLaunchKernelEx(&cfg, cache_combine_kernel<false, kCombineWarps>, P);
+  return bf16 ? cudaLaunchKernelEx(&cfg, cache_combine_kernel<true, 1>, P)
+              : cudaLaunchKernelEx(&cfg, cache_combine_kernel<false, 1>, P);
 }
 
 }  // namespace ra

@@ -8,14 +8,17 @@ constexpr int kAttendTile = 64;                // tokens per pipeline stage
 constexpr int kAttendWarps = 4;                // consumer warps, 16 tokens of a tile each
 constexpr int kAttendThreads = 32 * (kAttendWarps + 1);
 constexpr int kAttendMaxStages = 8;
+// What beginning and ending a work row costs, in tiles: loading its queries, merging the warps' sums.
+constexpr int kAttendRowUnits = 2;
 // CTAs per multiprocessor: three with 8 query columns (128 registers a thread), two with 16
 __host__ __device__ constexpr int attend_ctas(int nq) { return nq == 1 ? 3 : 2; }
 
 // One segment of the keys: the prefix (one cache, all batch rows' queries) or the rows' own caches.
-// A work row is (cache, kv head, tile of queries); its tiles of tokens lie one behind the other, and so
-// do the rows of a cache and the caches.  CTA c of the first G = min(grid, total) takes the tiles
-// [total c / G, total (c+1) / G) of that line, whatever rows they belong to, and leaves one partial for each row it touches, in slot row + c:
-// along the line one of the two grows at every step, so the slots are distinct.
+// A work row is (cache, kv head, tile of queries).  The rows lie on a line, one behind the other, cache
+// by cache, each as long as what it costs: kAttendRowUnits and then a unit for each tile of tokens.  CTA
+// c of the first G = min(grid, total) takes the units [total c / G, total (c+1) / G), whatever rows they
+// belong to, and leaves one partial for each row of which it has tiles, in slot row + c: along the line
+// one of the two grows at every step, so the slots are distinct.
 struct AttendSegment {
   CUtensorMap kmap, vmap;
   CacheView cache;
@@ -27,7 +30,7 @@ struct AttendSegment {
   int nstages;
   float* part_o;            // [slots][8 NQ][128] un-normalised sums
   float* part_ml;           // [slots][8 NQ][2] maximum (log2 domain), weight
-  long long* line;          // [caches + 1]: tiles of (kv head, query tile) before each cache
+  int* span;                // [rows][2]: first and last CTA with tiles of the row (of one with tokens)
 };
 
 struct CacheAttendParams {
@@ -36,13 +39,16 @@ struct CacheAttendParams {
   unsigned* status;
   int hq, hkv, group;
   float scale_log2e;
+  int after;                // launched while the prefix's kernel still runs: needs nothing of it, but
+                            // ends behind it, so that the combine need only wait for this one
 };
 
 // What the combine reads of a segment.
 struct CombineSegment {
   const float* part_o;      // null: no such segment
   const float* part_ml;
-  const long long* line;
+  const int* span;
+  const int* lens;
   int queries, query_tiles, qt, grid, prefix;
 };
 struct CombineParams {
