@@ -9,6 +9,7 @@
 
 #include "api_host.cuh"
 #include "cache_attend.cuh"
+#include "prefix_attend.cuh"
 
 namespace {
 
@@ -89,8 +90,9 @@ int check_rows(const ra_kv_rows_params* p, QuantParams& q) {
   return RA_OK;
 }
 
-// Tensor map over K or V: 64-token boxes of one head, swizzled over the 128 (int4: 64) bytes of a row.
-int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int format, int heads, int caches) {
+// Tensor map over K or V: boxes of `rows` tokens of one head, swizzled over the 128 (int4: 64) bytes of a
+// row or half row.
+int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int format, int heads, int caches, int rows) {
   EncodeTiledFn enc = host_encode_fn();
   if (!enc) return host_fail(RA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const bool dense = format <= RA_CACHE_BF16;
@@ -98,7 +100,7 @@ int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int forma
   const cuuint64_t dims[4] = {row, (cuuint64_t)heads, (cuuint64_t)v.n_tokens, (cuuint64_t)caches};
   const cuuint64_t strides[3] = {(cuuint64_t)v.hstride, (cuuint64_t)v.tstride,
                                  (cuuint64_t)(caches > 1 ? v.bstride : v.tstride)};
-  const cuuint32_t box[4] = {(cuuint32_t)(dense ? 64 : row), 1, (cuuint32_t)kAttendTile, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)(dense ? 64 : row), 1, (cuuint32_t)rows, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type = format == RA_CACHE_FP16   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                    : format == RA_CACHE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -119,13 +121,29 @@ int encode_map(CUtensorMap* map, const void* base, const CacheView& v, int forma
 
 // How one segment is worked on, and where its partials lie in the scratch.
 struct SegmentPlan {
-  int caches, queries, nq, query_tiles, grid;
+  int caches, queries, qt, query_tiles;
+  int nq, grid;        // of the line of work rows (cache_attend)
+  int splits;          // > 0: the prefix goes to prefix_attend, its tokens cut into so many ranges
   size_t ml_at, span_at, bytes;   // part_o at 0
 };
 
-constexpr int kMaxSms = 256;      // bound of the device-independent workspace size
+// Ranges that the prefix's tokens are cut into: the fewest rounds of CTAs, one to a multiprocessor, by
+// what each costs (its tiles, and about four for its beginning and end).
+int prefix_splits(int blocks, int tiles, int sms) {
+  int best = 1;
+  long long best_cost = -1;
+  for (int s = 1; s <= std::min(tiles, std::max(1, 2 * sms / blocks)); ++s) {
+    const long long rounds = ((long long)blocks * s + sms - 1) / sms;
+    const long long cost = rounds * ((tiles + s - 1) / s + 4);
+    if (best_cost < 0 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
 
-SegmentPlan plan_segment(bool prefix, int batch, int hq, int hkv, int tokens, int sms) {
+SegmentPlan plan_segment(bool prefix, bool dense, int batch, int hq, int hkv, int tokens, int sms) {
   SegmentPlan s;
   memset(&s, 0, sizeof s);
   if (tokens <= 0) return s;
@@ -133,14 +151,23 @@ SegmentPlan plan_segment(bool prefix, int batch, int hq, int hkv, int tokens, in
   s.caches = prefix ? 1 : batch;
   s.queries = prefix ? batch * group : group;
   s.nq = s.queries <= 8 ? 1 : 2;
-  s.query_tiles = (s.queries + 8 * s.nq - 1) / (8 * s.nq);
+  const bool wide = prefix && dense && s.queries > 16;
+  s.qt = wide ? kPrefixTile : 8 * s.nq;
+  s.query_tiles = (s.queries + s.qt - 1) / s.qt;
   const long long rows = (long long)s.caches * hkv * s.query_tiles;
-  const long long units = rows * ((tokens + kAttendTile - 1) / kAttendTile + kAttendRowUnits);
-  s.grid = (int)std::min<long long>(units, (long long)attend_ctas(s.nq) * sms);
-  const size_t slots = (size_t)rows + s.grid;
+  size_t slots;
+  if (wide) {
+    const int blocks = (s.query_tiles + 1) / 2 * hkv;
+    s.splits = prefix_splits(blocks, (tokens + kPrefixTile - 1) / kPrefixTile, sms);
+    slots = (size_t)rows * 2 * s.splits;
+  } else {
+    const long long units = rows * ((tokens + kAttendTile - 1) / kAttendTile + kAttendRowUnits);
+    s.grid = (int)std::min<long long>(units, (long long)attend_ctas(s.nq) * sms);
+    slots = (size_t)rows + s.grid;
+  }
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
-  s.ml_at = up(slots * 8 * s.nq * kHeadDim * sizeof(float));
-  s.span_at = s.ml_at + up(slots * 8 * s.nq * 2 * sizeof(float));
+  s.ml_at = up(slots * s.qt * kHeadDim * sizeof(float));
+  s.span_at = s.ml_at + up(slots * s.qt * 2 * sizeof(float));
   s.bytes = s.span_at + up((size_t)rows * 2 * sizeof(int));
   return s;
 }
@@ -176,8 +203,13 @@ int ra_kv_dequantize(const ra_kv_rows_params* p) {
 size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                           int32_t prefix_tokens, int32_t cache_tokens) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || prefix_tokens < 0 || cache_tokens < 0) return 0;
-  return 256 + plan_segment(true, batch, num_q_heads, num_kv_heads, prefix_tokens, kMaxSms).bytes +
-         plan_segment(false, batch, num_q_heads, num_kv_heads, cache_tokens, kMaxSms).bytes;
+  // room for either kind of cache
+  const int sms = host_sm_count();
+  size_t need = 0;
+  for (int dense = 0; dense < 2; ++dense)
+    need = std::max(need, plan_segment(true, dense, batch, num_q_heads, num_kv_heads, prefix_tokens, sms).bytes +
+                              plan_segment(false, dense, batch, num_q_heads, num_kv_heads, cache_tokens, sms).bytes);
+  return 256 + need;
 }
 
 int ra_cache_attention(const ra_cache_attention_params* p) {
@@ -209,7 +241,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
                      "workspace missing, misaligned or smaller than ra_cache_attention_workspace_bytes()");
   cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const bool bf16 = p->type == RA_TYPE_BF16;
-  const int sms = std::min(host_sm_count(), kMaxSms);
+  const int sms = host_sm_count();
   CombineParams cp;
   memset(&cp, 0, sizeof cp);
   cp.out = p->out;
@@ -221,13 +253,53 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;
     const int format = (i ? p->cache : p->prefix).format;
-    const SegmentPlan s = plan_segment(i == 0, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
+    const bool dense = format <= RA_CACHE_BF16;
+    const SegmentPlan s =
+        plan_segment(i == 0, dense, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
+    float* part_o = reinterpret_cast<float*>(at);
+    float* part_ml = reinterpret_cast<float*>(at + s.ml_at);
+    CombineSegment& c = cp.seg[i];
+    c.part_o = part_o;
+    c.part_ml = part_ml;
+    c.span = reinterpret_cast<int*>(at + s.span_at);
+    c.lens = i ? p->seq_lens : nullptr;
+    c.query_tiles = s.query_tiles;
+    c.qt = s.qt;
+    c.splits = s.splits;
+    c.prefix = i == 0;
+    at += s.bytes;
+    const int box = s.splits ? kPrefixTile : kAttendTile;
+    CUtensorMap maps[2];
+    for (int j = 0; j < 2; ++j) {
+      const int st = encode_map(&maps[j], j ? view[i].v : view[i].k, view[i], format, p->num_kv_heads, s.caches, box);
+      if (st != RA_OK) return st;
+    }
+    if (s.splits) {
+      PrefixAttendParams a;
+      memset(&a, 0, sizeof a);
+      a.kmap = maps[0];
+      a.vmap = maps[1];
+      a.q = p->q;
+      a.part_o = part_o;
+      a.part_ml = part_ml;
+      a.status = static_cast<unsigned*>(p->status);
+      a.n_tokens = view[i].n_tokens;
+      a.queries = s.queries;
+      a.query_tiles = s.query_tiles;
+      a.hq = p->num_q_heads;
+      a.hkv = p->num_kv_heads;
+      a.group = cp.group;
+      a.splits = s.splits;
+      a.scale_log2e = p->sm_scale * kLog2e;
+      const cudaError_t e = launch_prefix_attend(a, bf16, stream);
+      if (e != cudaSuccess) return host_cuda_fail(e, "prefix_attend launch");
+      continue;
+    }
     CacheAttendParams a;
     memset(&a, 0, sizeof a);
     AttendSegment& g = a.seg;
-    int st = encode_map(&g.kmap, view[i].k, view[i], format, p->num_kv_heads, s.caches);
-    if (st == RA_OK) st = encode_map(&g.vmap, view[i].v, view[i], format, p->num_kv_heads, s.caches);
-    if (st != RA_OK) return st;
+    g.kmap = maps[0];
+    g.vmap = maps[1];
     g.cache = view[i];
     g.lens = i ? p->seq_lens : nullptr;
     g.caches = s.caches;
@@ -235,9 +307,9 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
     g.query_tiles = s.query_tiles;
     g.grid = s.grid;
     g.nstages = cache_attend_stages(format, s.nq);
-    g.part_o = reinterpret_cast<float*>(at);
-    g.part_ml = reinterpret_cast<float*>(at + s.ml_at);
-    g.span = reinterpret_cast<int*>(at + s.span_at);
+    g.part_o = part_o;
+    g.part_ml = part_ml;
+    g.span = const_cast<int*>(c.span);
     a.q = p->q;
     a.status = static_cast<unsigned*>(p->status);
     a.hq = p->num_q_heads;
@@ -245,17 +317,6 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
     a.group = cp.group;
     a.after = i == 1 && has[0];
     a.scale_log2e = p->sm_scale * kLog2e;
-    CombineSegment& c = cp.seg[i];
-    c.part_o = g.part_o;
-    c.part_ml = g.part_ml;
-    c.span = g.span;
-    c.lens = g.lens;
-    c.queries = s.queries;
-    c.query_tiles = s.query_tiles;
-    c.qt = 8 * s.nq;
-    c.grid = s.grid;
-    c.prefix = i == 0;
-    at += s.bytes;
     const cudaError_t e = launch_cache_attend(a, format, bf16, s.nq, stream);
     if (e != cudaSuccess) return host_cuda_fail(e, "cache_attend launch");
   }

@@ -757,9 +757,16 @@ cache_combine_kernel(const __grid_constant__ CombineParams P) {
     const int qi = hq % P.group + (G.prefix ? b * P.group : 0);
     const long long row = (long long)cache * P.hkv * G.query_tiles + h * G.query_tiles + qi / G.qt;
     if (G.lens && G.lens[cache] <= 0) continue;
-    const int2 span = *reinterpret_cast<const int2*>(G.span + 2 * row);
+    int2 span;
+    long long slot0 = row;
+    if (G.splits) {
+      slot0 = row * 2 * G.splits;
+      span = make_int2(0, (((qi / G.qt) | 1) < G.query_tiles ? G.splits : 2 * G.splits) - 1);
+    } else {
+      span = *reinterpret_cast<const int2*>(G.span + 2 * row);
+    }
     const int c1 = span.y, per = min(32, (span.y - span.x + WARPS) / WARPS);
-    const long long e0 = row * G.qt + qi % G.qt;
+    const long long e0 = slot0 * G.qt + qi % G.qt;
     for (int c = span.x + per * (warp % WARPS); c <= c1; c += per * WARPS) {
       const int n = min(per, c1 - c + 1);
       float2 ml = make_float2(kNoMax, 0.f);

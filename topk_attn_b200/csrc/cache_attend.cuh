@@ -49,7 +49,9 @@ struct CombineSegment {
   const float* part_ml;
   const int* span;
   const int* lens;
-  int queries, query_tiles, qt, grid, prefix;
+  int query_tiles, qt, prefix;
+  int splits;               // > 0: a row's partials lie in 2 * splits slots of its own, of which a query
+                            // tile that has a partner uses the first half
 };
 struct CombineParams {
   CombineSegment seg[2];
