@@ -7,8 +7,8 @@
 // streams, each with its own S and O in TMEM and its own softmax warpgroup, so that the tensor cores
 // work on one while the other's softmax runs.  With two query tiles both streams walk the same K/V
 // tiles; with one, they take the tiles in turn and leave a partial each.
-//   warp 0      TMA: K and V tiles of 32 KiB in one ring, in the order of their first use
-//   warp 1      one thread issues the MMAs; its commits release tiles and hand over S
+//   warp 0      TMA: K and V tiles of 32 KiB in one ring
+//   warps 1, 2  one thread of each issues a stream's MMAs; its commits release tiles and hand over S
 //   warps 4-11  softmax: a thread owns one query (one TMEM lane), so maximum and sum need no exchange;
 //               P goes back into S's columns as the A operand of the second product
 // The maximum moves only when a score exceeds it by 2^4, and only then O is rescaled in TMEM; no wait
@@ -20,11 +20,13 @@ namespace ra {
 constexpr int kPrefixStages = 5;
 constexpr int kPrefixThreads = 384;
 constexpr int kPrefixSoftRegs = 232, kPrefixOtherRegs = 40;   // 256 * 232 + 128 * 40 = 384 * 168
+constexpr int kPrefixEarly = 64;                // tokens of P whose product starts while the rest is computed
+constexpr int kPrefixYield = 2;                 // quarter of P after which the other stream's turn begins
 constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f;
 
 struct PrefixCtrl {
   uint64_t full[kPrefixStages], empty[kPrefixStages];
-  uint64_t q_full, s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, s_full[2], p_full[2][2], o_full[2], turn[2], drain[2];
   uint32_t tmem;
   int timeout;
 };
@@ -59,6 +61,11 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "r"(a), "l"(b), "r"(idesc), "r"(add)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 #define RA_TC_R8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
 #define RA_TC_W8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
 // 32 consecutive columns of this thread's lane
@@ -75,6 +82,35 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
       "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::RA_TC_R8(v, 0),
       RA_TC_R8(v, 8), RA_TC_R8(v, 16), RA_TC_R8(v, 24), "r"(addr)
       : "memory");
+}
+
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::RA_TC_R8(v, 0),
+      RA_TC_R8(v, 8), "r"(addr)
+      : "memory");
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  Rows along K (Q, K tiles): groups of 8 rows are
@@ -116,21 +152,25 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   const int all_tiles = ceil_div(P.n_tokens, kPrefixTile);
   const int tile0 = (int)((long long)all_tiles * split / P.splits);
   const int tiles = (int)((long long)all_tiles * (split + 1) / P.splits) - tile0;
-  // step i: stream i & 1, tile i / 2 (two query tiles) or i (one)
-  const int steps = pair ? 2 * tiles : tiles;
+  // stream s walks the tiles s, s + 2, .. of one query tile, or all of them for query tile s; tile j's K
+  // is load 2 j of the ring, its V load 2 j + 1
+  const int stride = pair ? 1 : 2;
 
   if (tid == 0) {
     tma_prefetch_desc(&P.kmap);
     tma_prefetch_desc(&P.vmap);
     for (int s = 0; s < kPrefixStages; ++s) {
       mbar_init(&ctrl->full[s], 1);
-      mbar_init(&ctrl->empty[s], 1);
+      mbar_init(&ctrl->empty[s], pair ? 2 : 1);
     }
     mbar_init(&ctrl->q_full, 256);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctrl->s_full[s], 1);
-      mbar_init(&ctrl->p_full[s], 128);
+      mbar_init(&ctrl->p_full[s][0], 128);
+      mbar_init(&ctrl->p_full[s][1], 128);
       mbar_init(&ctrl->o_full[s], 1);
+      mbar_init(&ctrl->turn[s], 128);
+      mbar_init(&ctrl->drain[s], 1);
     }
     ctrl->timeout = 0;
     fence_barrier_init();
@@ -141,10 +181,12 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = ctrl->tmem;
-  auto tm_s = [&](int stream) { return tmem + 128u * stream; };          // S, then P in its first half
-  auto tm_o = [&](int stream) { return tmem + 256u + 128u * stream; };
+  // TMEM columns of stream st: S at 128 st, P in its first half; O at 256 + 128 st
+  // false: a wait ran out, here or elsewhere in the CTA; the role that sees it stops
   auto wait = [&](uint64_t* bar, unsigned parity) {
-    if (!mbar_wait(bar, parity, &ctrl->timeout)) atomicOr(P.status, kStatusTimeout);
+    if (mbar_wait(bar, parity, &ctrl->timeout)) return true;
+    atomicOr(P.status, kStatusTimeout);
+    return false;
   };
 
   if (warp < 4) {
@@ -152,62 +194,86 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA
       int n = 0;
-      auto load = [&](const CUtensorMap* map, int tile) {
+      for (; n < 2 * tiles; ++n) {
         const int s = n % kPrefixStages;
-        wait(&ctrl->empty[s], ((n / kPrefixStages) & 1) ^ 1);
+        if (!wait(&ctrl->empty[s], ((n / kPrefixStages) & 1) ^ 1)) break;
         unsigned char* dst = sm_kv + s * kPrefixTileBytes;
-        const int tok = (tile0 + tile) * kPrefixTile;
+        const CUtensorMap* map = (n & 1) ? &P.vmap : &P.kmap;
+        const int tok = (tile0 + (n >> 1)) * kPrefixTile;
         mbar_expect_tx(&ctrl->full[s], kPrefixTileBytes);
         tma_load_4d(dst, map, &ctrl->full[s], 0, h, tok, 0);
         tma_load_4d(dst + kPrefixHalf, map, &ctrl->full[s], 64, h, tok, 0);
-        ++n;
-      };
-      load(&P.kmap, 0);
-      if (!pair && steps > 1) load(&P.kmap, 1);
-      for (int i = 0; i < steps; ++i) {
-        const bool fresh = !pair || !(i & 1);
-        const int j = pair ? i >> 1 : i, ahead = pair ? j + 1 : j + 2;
-        if (fresh) load(&P.vmap, j);
-        if (fresh && ahead < tiles) load(&P.kmap, ahead);
       }
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------------- MMA
+      // after a wait that ran out: no load may still be under way when the CTA ends
+      if (n < 2 * tiles) {
+        int own = 0;
+        for (int i = max(0, n - kPrefixStages); i < n; ++i)
+          mbar_wait(&ctrl->full[i % kPrefixStages], (i / kPrefixStages) & 1, &own);
+      }
+    } else if (warp == 1 || warp == 2) {
+      // ---------------------------------------------------------------- MMA, stream warp - 1
+      // The whole warp walks the steps, so that descriptors and addresses are uniform values; one
+      // elected thread issues.  (From a branch of one lane every MMA took about 100 cycles to issue, and
+      // with one warp for both streams each stream waited for the other's issue.)
       constexpr uint32_t kIdS = tc_idesc(BF16, false), kIdO = tc_idesc(BF16, true);
-      int n = 0, ks = 0, vs = 0;
-      const uint32_t kv = smem_u32(sm_kv), sq = smem_u32(sm_q);
-      auto take = [&]() {
-        const int s = n % kPrefixStages;
-        wait(&ctrl->full[s], (n / kPrefixStages) & 1);
-        ++n;
-        return s;
-      };
-      auto scores = [&](int i) {
-        const bool fresh = !pair || !(i & 1);
-        if (fresh) ks = take();
+      const int st = warp - 1;
+      const uint32_t tm_s = __shfl_sync(0xffffffffu, tmem, 0) + 128u * st, tm_o = tm_s + 256u;
+      const uint64_t q_desc = tc_desc(smem_u32(sm_q) + (pair ? st * kPrefixTileBytes : 0), 16, 1024);
+      const uint64_t k_desc = tc_desc(smem_u32(sm_kv), 16, 1024);
+      const uint64_t v_desc = tc_desc(smem_u32(sm_kv), kPrefixHalf, 1024);
+      auto ready = [&](int n) { return wait(&ctrl->full[n % kPrefixStages], (n / kPrefixStages) & 1); };
+      auto scores = [&](int j) {
+        const int s = 2 * j % kPrefixStages;
+        const uint64_t b = k_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         tc_fence_after();
-        const uint32_t a = sq + (pair ? (i & 1) * kPrefixTileBytes : 0), b = kv + ks * kPrefixTileBytes;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kPrefixHalf + (k & 3) * 32;
-          tc_mma_ss(tm_s(i & 1), tc_desc(a + off, 16, 1024), tc_desc(b + off, 16, 1024), kIdS, k > 0);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t off = ((k >> 2) * kPrefixHalf + (k & 3) * 32) >> 4;
+            tc_mma_ss(tm_s, q_desc + off, b + off, kIdS, k > 0);
+          }
+          tc_commit(&ctrl->empty[s]);
+          tc_commit(&ctrl->s_full[st]);
         }
-        if (!pair || (i & 1)) tc_commit(&ctrl->empty[ks]);
-        tc_commit(&ctrl->s_full[i & 1]);
+        __syncwarp();
       };
-      wait(&ctrl->q_full, 0);
-      scores(0);
-      if (steps > 1) scores(1);
-      for (int i = 0; i < steps; ++i) {
-        if (!pair || !(i & 1)) vs = take();
-        wait(&ctrl->p_full[i & 1], (i >> 1) & 1);
+      int j = pair ? 0 : st;
+      bool ok = wait(&ctrl->q_full, 0) && (j >= tiles || ready(2 * j));
+      if (ok && j < tiles) scores(j);
+      for (unsigned k = 0; ok && j < tiles; j += stride, ++k) {
+        // the tiles first, so that the products follow one another once P is there
+        const bool more = j + stride < tiles;
+        ok = ready(2 * j + 1) && (!more || ready(2 * (j + stride)));
+        const int s = (2 * j + 1) % kPrefixStages;
+        const uint64_t b = v_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
+        ok = ok && wait(&ctrl->p_full[st][0], k & 1);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t b = kv + vs * kPrefixTileBytes;
+        const uint32_t add = k > 0;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          tc_mma_ts(tm_o(i & 1), tm_s(i & 1) + 8 * k, tc_desc(b + k * 2048, kPrefixHalf, 1024), kIdO, i > 1 || k > 0);
-        if (!pair || (i & 1)) tc_commit(&ctrl->empty[vs]);
-        if (i + 2 >= steps) tc_commit(&ctrl->o_full[i & 1]);
-        if (i + 2 < steps) scores(i + 2);
+          for (int c = 0; c < kPrefixEarly / 16; ++c)
+            tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, c > 0 ? 1u : add);
+        }
+        __syncwarp();
+        ok = wait(&ctrl->p_full[st][1], k & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int c = kPrefixEarly / 16; c < 8; ++c)
+            tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+          tc_commit(&ctrl->empty[s]);
+          if (!more) tc_commit(&ctrl->o_full[st]);
+        }
+        __syncwarp();
+        if (more) scores(j + stride);
+      }
+      if (!ok) {   // no product may still be under way when TMEM is given back
+        if (elect_one()) tc_commit(&ctrl->drain[st]);
+        __syncwarp();
+        int own = 0;
+        mbar_wait(&ctrl->drain[st], 0, &own, kWaitLimitNs / 4);
       }
     }
     __syncwarp();
@@ -217,28 +283,43 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     const int st = (warp >> 2) - 1;           // stream
     const int soft = tid - 128;
     {
-      const int rows = pair ? 256 : 128;
-      const int c = soft & 15;
-#pragma unroll 4
-      for (int r = soft >> 4; r < rows; r += 16) {
-        const int qi = qt0 * kPrefixTile + r;
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (qi < P.queries) {
-          const long long row = (long long)(qi / P.group) * P.hq + h * P.group + qi % P.group;
-          u = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(P.q) + row * kRowBytes + 16 * c);
+      // 16 lanes to a row; all of a thread's loads are under way before the first is stored
+      const int c = soft & 15, n = pair ? 16 : 8;
+      const int first = qt0 * kPrefixTile + (soft >> 4);
+      const int step_b = 16 / P.group, step_g = 16 % P.group;
+      int qb = first / P.group, qg = first % P.group;
+      uint4 u[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        u[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < n && first + 16 * i < P.queries) {
+          const long long row = (long long)qb * P.hq + h * P.group + qg;
+          u[i] = ldg128_nc(static_cast<const unsigned char*>(P.q) + row * kRowBytes + 16 * c);
         }
-        *reinterpret_cast<uint4*>(sm_q + (r >> 7) * kPrefixTileBytes + swz128(r & 127, c)) = u;
+        qb += step_b;
+        qg += step_g;
+        if (qg >= P.group) {
+          qg -= P.group;
+          ++qb;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = (soft >> 4) + 16 * i;
+        if (i < n) *reinterpret_cast<uint4*>(sm_q + (r >> 7) * kPrefixTileBytes + swz128(r & 127, c)) = u[i];
       }
       fence_proxy_async();
       mbar_arrive(&ctrl->q_full);
     }
     // ---------------------------------------------------------------- softmax
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;    // my warp's 32 TMEM lanes
-    const uint32_t tms = tm_s(st) + lanes, tmo = tm_o(st) + lanes;
+    const uint32_t tms = tmem + 128u * st + lanes, tmo = tms + 256u;
     float m_ref = kPfNoMax, l = 0.f;
     int k = 0;
-    for (int i = st; i < steps; i += 2, ++k) {
-      wait(&ctrl->s_full[st], k & 1);
+    bool ok = true;
+    for (int j = pair ? 0 : st; j < tiles; j += stride, ++k) {
+      ok = __all_sync(0xffffffffu, wait(&ctrl->s_full[st], k & 1));
+      if (!ok) break;
       tc_fence_after();
       uint32_t s[128];
       tc_ld32(s, tms);
@@ -246,8 +327,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       tc_ld32(s + 64, tms + 64);
       tc_ld32(s + 96, tms + 96);
       tc_wait_ld();
-      const int tile = tile0 + (pair ? i >> 1 : i);
-      const int valid = P.n_tokens - tile * kPrefixTile;
+      const int valid = P.n_tokens - (tile0 + j) * kPrefixTile;
       if (valid < kPrefixTile) {
 #pragma unroll
         for (int c = 0; c < 128; ++c)
@@ -258,7 +338,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       for (int c = 0; c < 128; c += 8)
 #pragma unroll
         for (int d = 0; d < 4; ++d)
-          mx4[d] = fmaxf(mx4[d], fmaxf(__uint_as_float(s[c + d]), __uint_as_float(s[c + d + 4])));
+          mx4[d] = max3(mx4[d], __uint_as_float(s[c + d]), __uint_as_float(s[c + d + 4]));
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * P.scale_log2e;
       if (__any_sync(0xffffffffu, mx > m_ref + (kPfLazy + kPfLift))) {
         const float m_new = fmaxf(m_ref, mx - kPfLift), alpha = fast_exp2(m_ref - m_new);
@@ -276,35 +356,50 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
           }
         }
       }
-      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+      // the streams take turns at the exponentials: left alone they fall into step, and then the
+      // tensor cores idle while both compute, and the other way round
+      if (st ? true : k > 0) ok = __all_sync(0xffffffffu, wait(&ctrl->turn[st], (st ? k : k - 1) & 1));
+      if (!ok) break;
+      const float2 scale2 = make_float2(P.scale_log2e, P.scale_log2e), neg_m = make_float2(-m_ref, -m_ref);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
+      for (int part = 0; part < 4; ++part) {
+        uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float a = fast_exp2(__fmaf_rn(__uint_as_float(s[64 * half + 2 * c]), P.scale_log2e, -m_ref));
-          const float b = fast_exp2(__fmaf_rn(__uint_as_float(s[64 * half + 2 * c + 1]), P.scale_log2e, -m_ref));
-          l4[(2 * c) & 3] += a;
-          l4[(2 * c + 1) & 3] += b;
-          p[c] = pf_pack<BF16>(a, b);
+        for (int c = 0; c < 16; ++c) {
+          const int e = 32 * part + 2 * c;
+          float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, neg_m);
+          x.x = fast_exp2(x.x);
+          x.y = fast_exp2(x.y);
+          sum[c & 1] = add2(sum[c & 1], x);
+          p[c] = pf_pack<BF16>(x.x, x.y);
         }
-        tc_st32(tms + 32 * half, p);
+        tc_st16(tms + 16 * part, p);
+        if (part == kPrefixYield) mbar_arrive(&ctrl->turn[st ^ 1]);
+        if (part == kPrefixEarly / 32 - 1 || part == 3) {
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(&ctrl->p_full[st][part == 3]);
+        }
       }
-      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-      tc_wait_st();
-      tc_fence_before();
-      mbar_arrive(&ctrl->p_full[st]);
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     // ---------------------------------------------------------------- partial
     const int qt = pair ? qt0 + st : qt0;
     const long long slot = ((long long)h * P.query_tiles + qt) * (2 * P.splits) + (pair ? split : 2 * split + st);
-    const int row = (warp & 3) * 32 + lane;
-    float* out = P.part_o + (slot * kPrefixTile + row) * kHeadDim;
-    if (k) {
+    const int row0 = (warp & 3) * 32;                      // my warp's rows
+    if (k && ok) {
       wait(&ctrl->o_full[st], 0);
+      __syncwarp();
       tc_fence_after();
     }
-#pragma unroll
+    // 32 rows x 32 dims at a time through shared memory, so that rows leave in whole lines.  The query
+    // tile is free: with one tile the other's place is used, where no product reads.
+    const uint32_t buf = smem_u32(sm_q) + (pair ? st * kPrefixTileBytes + (warp & 3) * 4096
+                                                : kPrefixTileBytes + (warp - 4) * 4096);
+    const int live = P.queries - qt * kPrefixTile - row0;  // rows of mine that are queries
+    float* out = P.part_o + (slot * kPrefixTile + row0) * kHeadDim;
+#pragma unroll 1
     for (int c = 0; c < 128; c += 32) {
       uint32_t o[32];
       if (k) {
@@ -314,14 +409,21 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
         for (int d = 0; d < 32; ++d) o[d] = 0u;
       }
-      if (qt * kPrefixTile + row < P.queries) {
 #pragma unroll
-        for (int d = 0; d < 32; d += 4)
-          *reinterpret_cast<uint4*>(out + c + d) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+      for (int d = 0; d < 8; ++d)
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(buf + lane * 128 + ((d ^ (lane & 7)) << 4)),
+                     "r"(o[4 * d]), "r"(o[4 * d + 1]), "r"(o[4 * d + 2]), "r"(o[4 * d + 3])
+                     : "memory");
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), d = lane & 7;
+        const uint4 v = lds128(buf + r * 128 + ((d ^ (r & 7)) << 4));
+        if (r < live) *reinterpret_cast<uint4*>(out + r * kHeadDim + c + 4 * d) = v;
       }
+      __syncwarp();
     }
-    float* ml = P.part_ml + (slot * kPrefixTile + row) * 2;
-    *reinterpret_cast<float2*>(ml) = make_float2(m_ref, l);
+    *reinterpret_cast<float2*>(P.part_ml + (slot * kPrefixTile + row0 + lane) * 2) = make_float2(m_ref, l);
     tc_fence_before();
   }
   __syncthreads();
