@@ -82,23 +82,31 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-def extension_path() -> str:
+def extension_path(name: str = "retrieval_attention_cpp") -> str:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    return os.path.join(PKG, "retrieval_attention_cpp" + suffix)
+    return os.path.join(PKG, name + suffix)
 
 
 def build_extension(force: bool = False) -> str:
-    """Compile bind.cpp against torch's headers and link it to the C-ABI library."""
+    """Compile the torch bindings (bind.cpp, cache_bind.cpp) and link them to the C-ABI library."""
+    jobs = [_build_binding(src, name, force) for src, name in
+            (("bind.cpp", "retrieval_attention_cpp"), ("cache_bind.cpp", "cache_ops_cpp"))]
+    for job in jobs:
+        if job is not None and job.wait() != 0:
+            raise RuntimeError("g++ failed on a torch binding")
+    return extension_path()
+
+
+def _build_binding(source: str, name: str, force: bool):
     import torch
     from torch.utils import cpp_extension as ce
 
-    out = extension_path()
-    src = os.path.join(CSRC, "bind.cpp")
+    src, out = os.path.join(CSRC, source), extension_path(name)
     if not force and not _newer(out, [src, LIB, os.path.join(ROOT, "include", "topk_attn_b200.h")]):
-        return out
+        return None
     inc = ce.include_paths()
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", out,
-           "-DTORCH_EXTENSION_NAME=retrieval_attention_cpp", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
            "-I", "/usr/local/cuda/include"]
@@ -108,8 +116,7 @@ def build_extension(force: bool = False) -> str:
     cmd += ["-L", tlib, "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
             "-L", LIBDIR, "-ltopk_attn_b200",
             f"-Wl,-rpath,{tlib}", "-Wl,-rpath,$ORIGIN/lib", f"-Wl,-rpath,{LIBDIR}"]
-    subprocess.check_call(cmd)
-    return out
+    return subprocess.Popen(cmd)
 
 
 def build_cli(force: bool = False) -> str:

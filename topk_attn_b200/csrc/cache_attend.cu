@@ -20,6 +20,8 @@
 // HBM-bound: 264 bytes per token and kv head in 8 bits, 160 in 4, 512 in 16.
 #include "cache_attend.cuh"
 
+#include "api_host.cuh"
+
 namespace ra {
 
 template <int NQ>
@@ -828,7 +830,8 @@ template <int FMT, bool BF16, int NQ>
 cudaError_t launch_one(const CacheAttendParams& P, cudaStream_t stream) {
   auto kern = cache_attend_kernel<FMT, BF16, NQ>;
   const size_t smem = (size_t)P.seg.nstages * stage_bytes(FMT) + kMergeBytes + sizeof(AttendCtrl<NQ>) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)P.seg.grid);

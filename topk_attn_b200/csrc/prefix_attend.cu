@@ -15,6 +15,8 @@
 // is needed for that: S(k) is committed after O's product k-1.  Weights are rounded to the type of V.
 #include "prefix_attend.cuh"
 
+#include "api_host.cuh"
+
 namespace ra {
 
 constexpr int kPrefixStages = 5;
@@ -434,7 +436,8 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 cudaError_t launch_prefix_attend(const PrefixAttendParams& P, bool bf16, cudaStream_t stream) {
   auto kern = bf16 ? prefix_attend_kernel<true> : prefix_attend_kernel<false>;
   const size_t smem = (size_t)(2 + kPrefixStages) * kPrefixTileBytes + sizeof(PrefixCtrl) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> done[2];
+  const cudaError_t e = allow_smem(kern, smem, done[bf16]);
   if (e != cudaSuccess) return e;
   const int blocks = (P.query_tiles + 1) / 2 * P.hkv * P.splits;
   note_launch();

@@ -323,121 +323,17 @@ def quantized_kv_cache(num_tokens: int, num_kv_heads: int, kind: str = "int8", b
                        *(torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2)))
 
 
-_ROW_TYPES = {torch.float16: capi.RA_TYPE_FP16, torch.bfloat16: capi.RA_TYPE_BF16}
-_CODE_FORMATS = {torch.int8: capi.RA_CACHE_INT8, torch.float8_e4m3fn: capi.RA_CACHE_FP8,
-                 torch.uint8: capi.RA_CACHE_INT4}
-_status_blocks: Dict[int, Tensor] = {}
+_cache_binding = None
 
 
-def _status_block(device: torch.device) -> Tensor:
-    """The zeroed status block of ``device`` that ``check_status`` reads.  A graph captured before any
-    eager call on the device gets a block of its own, which ``check_status`` does not see."""
-    st = _status_blocks.get(device.index)
-    if st is None:
-        st = torch.zeros(256, dtype=torch.uint8, device=device)
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(device).synchronize()   # other streams use it from now on
-            _status_blocks[device.index] = st
-    return st
-
-
-def _scratch(nbytes: int, device: torch.device) -> Tensor:
-    """Scratch for one call: the stream's cached workspace behind its status block, or memory of its
-    own inside a capture (two captured graphs may be replayed at the same time, on any streams)."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return workspace(nbytes + 256, device)[256:]
-
-
-def _dense_strides(t: Tensor, row: int) -> Tuple[int, int, int]:
-    """(batch, token, head) strides of rows [B,T,H,row] or [T,H,row]; dimensions of size one, whose
-    stride means nothing, get the one a dense tensor would have."""
-    if t.stride(-1) != 1 and t.size(-1) != 1:
-        raise ValueError("the last dimension must be contiguous")
-    hs = t.stride(-2) if t.size(-2) > 1 else row
-    ts = t.stride(-3) if t.size(-3) > 1 else max(t.size(-2) * hs, row)
-    if t.dim() == 4 and t.size(0) > 1:
-        return t.stride(0), ts, hs
-    return max(t.size(-3), 1) * ts, ts, hs
-
-
-def _kv_cache(cache, per_row: bool, device: torch.device) -> Tuple[capi.RaKvCache, int, int]:
-    """(struct, caches, kv heads) of a QuantizedKV or a pair of fp16/bf16 tensors."""
-    c = capi.RaKvCache()
-    quantized = isinstance(cache, QuantizedKV)
-    k, v = (cache.k, cache.v) if quantized else cache
-    if k.dim() != (4 if per_row else 3) or v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("k and v must be [B,N,Hkv,128]" if per_row else "k and v must be [N,Hkv,128]")
-    if quantized:
-        if k.dtype not in _CODE_FORMATS:
-            raise ValueError("codes must be int8, float8_e4m3fn or uint8 (two int4)")
-        c.format = _CODE_FORMATS[k.dtype]
-    else:
-        if k.dtype not in _ROW_TYPES:
-            raise ValueError("caches must be fp16, bf16 or a QuantizedKV")
-        c.format = _ROW_TYPES[k.dtype]
-    int4 = c.format == capi.RA_CACHE_INT4
-    row = 64 if int4 else 128
-    if k.size(-1) != row:
-        raise ValueError(f"rows of this cache must have {row} elements")
-    caches, n, heads = (k.size(0) if per_row else 1), k.size(-3), k.size(-2)
-    for t in (k, v) + ((cache.k_scale, cache.v_scale) if quantized else ()):
-        if t.device != device:
-            raise ValueError("tensors must be on one CUDA device")
-    c.num_tokens = n
-    if n == 0:
-        return c, caches, heads
-    c.batch_stride, c.token_stride, c.head_stride = _dense_strides(k, row)
-    if _dense_strides(v, row) != (c.batch_stride, c.token_stride, c.head_stride):
-        raise ValueError("k and v must have the same strides")
-    c.k, c.v = k.data_ptr(), v.data_ptr()
-    if quantized:
-        ks, vs = cache.k_scale, cache.v_scale
-        want = ((caches,) if per_row else ()) + (heads, n) + ((4,) if int4 else ())
-        for t in (ks, vs):
-            if t.dtype != torch.float32 or tuple(t.shape) != want:
-                raise ValueError(f"scales must be fp32 {list(want)}")
-            if (n > 1 and t.stride(-2 if int4 else -1) != (4 if int4 else 1)) or (int4 and t.stride(-1) != 1):
-                raise ValueError("a head's scales must be contiguous along the tokens")
-
-        def lead(t):
-            hd = 1 if per_row else 0
-            hs = t.stride(hd) if heads > 1 else n * (4 if int4 else 1)
-            return (t.stride(0) if per_row and caches > 1 else heads * hs), hs
-        c.scale_batch_stride, c.scale_head_stride = lead(ks)
-        if lead(vs) != lead(ks):
-            raise ValueError("the scales of k and v must have the same strides")
-        c.k_scale, c.v_scale = ks.data_ptr(), vs.data_ptr()
-    return c, caches, heads
-
-
-def _int32_vector(t: Tensor, n: int, device: torch.device, name: str) -> int:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on the device of the others")
-    return t.data_ptr()
-
-
-def _kv_rows(cache: QuantizedKV, k: Tensor, v: Tensor, position, counts: Optional[Tensor]) -> capi.RaKvRowsParams:
-    dev = k.device
-    p = capi.RaKvRowsParams()
-    p.cache, p.caches, p.num_kv_heads = _kv_cache(cache, cache.per_row, dev)
-    if k.dim() != cache.k.dim() or k.size(-1) != 128 or k.size(-2) != p.num_kv_heads or v.shape != k.shape \
-            or (cache.per_row and k.size(0) != p.caches):
-        raise ValueError("rows must be [B,T,Hkv,128] for per-row caches, [T,Hkv,128] for a shared one")
-    if k.dtype not in _ROW_TYPES or v.dtype != k.dtype or v.device != dev:
-        raise ValueError("rows must be fp16 or bf16 tensors on the device of the cache")
-    p.head_dim, p.row_type, p.num_rows = 128, _ROW_TYPES[k.dtype], k.size(-3)
-    p.k_batch_stride, p.k_token_stride, p.k_head_stride = _dense_strides(k, 128)
-    p.v_batch_stride, p.v_token_stride, p.v_head_stride = _dense_strides(v, 128)
-    p.k_rows, p.v_rows = k.data_ptr(), v.data_ptr()
-    if isinstance(position, Tensor):
-        p.positions = _int32_vector(position, p.caches, dev, "position")
-    else:
-        p.position = int(position)
-    if counts is not None:
-        p.counts = _int32_vector(counts, p.caches, dev, "counts")
-    p.status, p.stream = _status_block(dev).data_ptr(), _stream_ptr()
-    return p
+def _cache_ops():
+    """The binding of the cache operators: it checks the tensors and fills the C ABI's structs."""
+    global _cache_binding
+    if _cache_binding is None:
+        from . import load_extension
+        capi.lib()
+        _cache_binding = load_extension("cache_ops_cpp")
+    return _cache_binding
 
 
 def kv_append_quantized(cache: QuantizedKV, new_k: Tensor, new_v: Tensor, position: Union[int, Tensor],
@@ -450,12 +346,10 @@ def kv_append_quantized(cache: QuantizedKV, new_k: Tensor, new_v: Tensor, positi
     device; ``counts`` int32 [B] says how many of the T rows of each are written (a padded batch).
     Rows that a device-side position puts outside the cache are left out and reported by
     ``check_status``."""
-    if not new_k.is_cuda:
-        raise ValueError("tensors must be CUDA tensors")
-    if new_k.dim() >= 3 and new_k.size(-3) == 0:
-        return
-    with torch.cuda.device(new_k.device):
-        capi.check(capi.lib().ra_kv_append_quantized(C.byref(_kv_rows(cache, new_k, new_v, position, counts))))
+    at, pos = (position, 0) if isinstance(position, Tensor) else (None, int(position))
+    st = _cache_ops().kv_rows(False, cache.k, cache.v, cache.k_scale, cache.v_scale, new_k, new_v, at, pos, counts)
+    if st:
+        capi.check(st)
 
 
 def kv_dequantize(cache: QuantizedKV, position: Union[int, Tensor] = 0, count: Optional[int] = None,
@@ -464,65 +358,42 @@ def kv_dequantize(cache: QuantizedKV, position: Union[int, Tensor] = 0, count: O
     tensors [B,count,Hkv,128] ([count,Hkv,128] for a shared cache).  ``position`` is as in
     ``kv_append_quantized``; ``count`` defaults to all tokens behind an int position.  Tokens that a
     device-side position puts outside the cache read as zeros and are reported by ``check_status``."""
-    if dtype not in _ROW_TYPES:
+    if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("dtype must be float16 or bfloat16")
     if not cache.k.is_cuda:
         raise ValueError("tensors must be CUDA tensors")
+    at, pos = (position, 0) if isinstance(position, Tensor) else (None, int(position))
     if count is None:
-        if isinstance(position, Tensor):
+        if at is not None:
             raise ValueError("a position on the device needs a count")
-        count = cache.num_tokens - position
+        count = cache.num_tokens - pos
     if count < 0:
         raise ValueError("count must not be negative")
     shape = (*cache.k.shape[:-3], count, cache.k.size(-2), 128)
-    with torch.cuda.device(cache.k.device):
-        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
-        if count:
-            capi.check(capi.lib().ra_kv_dequantize(C.byref(_kv_rows(cache, k, v, position, None))))
+    k, v = torch.empty(shape, dtype=dtype, device=cache.k.device), torch.empty(shape, dtype=dtype, device=cache.k.device)
+    st = _cache_ops().kv_rows(True, cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, at, pos, None)
+    if st:
+        capi.check(st)
     return k, v
+
+
+_NO_CACHE = (None, None, None, None)
+
+
+def _cache_tensors(cache) -> tuple:
+    if cache is None:
+        return _NO_CACHE
+    if isinstance(cache, QuantizedKV):
+        return cache.k, cache.v, cache.k_scale, cache.v_scale
+    k, v = cache
+    return k, v, None, None
 
 
 def _cache_attention(q: Tensor, prefix, cache, sm_scale: float, seq_lens: Optional[Tensor],
                      out: Optional[Tensor]) -> Tensor:
-    if not q.is_cuda:
-        raise ValueError("tensors must be CUDA tensors")
-    if q.dim() != 3 or q.size(2) != 128 or q.dtype not in _ROW_TYPES or not q.is_contiguous():
-        raise ValueError("q must be a contiguous fp16 or bf16 tensor [B,Hq,128]")
-    dev = q.device
-    B, Hq, _ = q.shape
-    if prefix is None and cache is None:
-        raise ValueError("nothing to attend to: give a prefix, a cache or both")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of the shape and type of q")
-    with torch.cuda.device(dev):
-        p = capi.RaCacheAttentionParams()
-        p.q, p.out, p.type = q.data_ptr(), out.data_ptr(), _ROW_TYPES[q.dtype]
-        p.batch, p.num_q_heads, p.head_dim = B, Hq, 128
-        heads = []
-        if prefix is not None:
-            p.prefix, _, h = _kv_cache(prefix, False, dev)
-            heads.append(h)
-        if cache is not None:
-            p.cache, caches, h = _kv_cache(cache, True, dev)
-            heads.append(h)
-            if caches != B:
-                raise ValueError("each row needs a cache: cache.size(0) must be the batch")
-        if len(set(heads)) != 1:
-            raise ValueError("prefix and cache must have the same kv heads")
-        p.num_kv_heads = heads[0]
-        if seq_lens is not None:
-            if cache is None:
-                raise ValueError("seq_lens are the lengths of the rows' own caches")
-            p.seq_lens = _int32_vector(seq_lens, B, dev, "seq_lens")
-        p.sm_scale = sm_scale
-        need = capi.lib().ra_cache_attention_workspace_bytes(B, Hq, p.num_kv_heads, p.prefix.num_tokens,
-                                                             p.cache.num_tokens)
-        ws = _scratch(max(need, 256), dev)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-        p.status, p.stream = _status_block(dev).data_ptr(), _stream_ptr()
-        capi.check(capi.lib().ra_cache_attention(C.byref(p)))
+    st, out = _cache_ops().cache_attention(q, *_cache_tensors(prefix), *_cache_tensors(cache), seq_lens, sm_scale, out)
+    if st:
+        capi.check(st)
     return out
 
 
@@ -714,12 +585,19 @@ def exchange_wait(flags: Tensor, epoch: Tensor, advance: bool, timeout_s: float 
                                            _stream_ptr()))
 
 
+def _cache_status(dev: torch.device) -> Optional[Tensor]:
+    """The status block that the cache operators share on a device, if one of them has run there."""
+    if _cache_binding is None:
+        return None
+    return _cache_binding.status_block(dev.index if dev.index is not None else torch.cuda.current_device())
+
+
 def check_status(device: Optional[torch.device] = None) -> None:
     """Synchronise the current stream and raise if a kernel abandoned a bounded wait."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     ws = workspace(256, dev)
     capi.check(capi.lib().ra_check_status(ws.data_ptr(), _stream_ptr()))
-    st = _status_blocks.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    st = _cache_status(dev)
     if st is not None:
         capi.check(capi.lib().ra_check_status(st.data_ptr(), _stream_ptr()))
 
@@ -728,6 +606,6 @@ def clear_status(device: Optional[torch.device] = None) -> None:
     """Reset the sticky bits that ``check_status`` reports, in order of the current stream."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     workspace(256, dev)[:256].zero_()
-    st = _status_blocks.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    st = _cache_status(dev)
     if st is not None:
         st.zero_()
