@@ -61,6 +61,8 @@ int check_rows(const ra_kv_rows_params* p, QuantParams& q) {
   if (!p) return invalid("params is null");
   if (p->head_dim != kHeadDim) return unsupported("head_dim must be 128");
   if (p->caches < 1 || p->num_kv_heads < 1 || p->num_rows < 0) return invalid("sizes must be positive");
+  if (p->caches > 65535 || p->num_kv_heads > kQuantMaxHeads)
+    return unsupported("more than 65535 caches or 1024 kv heads");
   if (p->cache.num_tokens < 1) return invalid("the cache has no tokens");
   if (p->cache.format < RA_CACHE_INT8) return invalid("the cache must be int8, fp8 or int4");
   if (p->row_type != RA_TYPE_FP16 && p->row_type != RA_TYPE_BF16) return invalid("rows must be fp16 or bf16");

@@ -29,11 +29,14 @@ struct CacheView {
   long long sbstride, shstride;
 };
 
+constexpr int kQuantMaxHeads = 1024;
+
 struct QuantParams {
   CacheView cache;
   void* rows[2];            // K and V rows, fp16 or bf16
   long long rb[2], rt[2], rh[2];   // their strides in elements
   int caches, heads, n_rows;
+  int tile;                 // tokens of a CTA (set by the launch)
   const int* positions;     // [caches] or null
   int position;
   const int* counts;        // [caches] or null
