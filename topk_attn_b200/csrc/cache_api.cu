@@ -145,7 +145,7 @@ int prefix_splits(int blocks, int tiles, int sms) {
   return best;
 }
 
-SegmentPlan plan_segment(bool prefix, bool dense, int batch, int hq, int hkv, int tokens, int sms) {
+SegmentPlan plan_segment(bool prefix, int format, int batch, int hq, int hkv, int tokens, int sms) {
   SegmentPlan s;
   memset(&s, 0, sizeof s);
   if (tokens <= 0) return s;
@@ -153,7 +153,7 @@ SegmentPlan plan_segment(bool prefix, bool dense, int batch, int hq, int hkv, in
   s.caches = prefix ? 1 : batch;
   s.queries = prefix ? batch * group : group;
   s.nq = s.queries <= 8 ? 1 : 2;
-  const bool wide = prefix && dense && s.queries > 16;
+  const bool wide = prefix && format != RA_CACHE_INT4 && s.queries > 16;
   s.qt = wide ? kPrefixTile : 8 * s.nq;
   s.query_tiles = (s.queries + s.qt - 1) / s.qt;
   const long long rows = (long long)s.caches * hkv * s.query_tiles;
@@ -208,9 +208,9 @@ size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, in
   // room for either kind of cache
   const int sms = host_sm_count();
   size_t need = 0;
-  for (int dense = 0; dense < 2; ++dense)
-    need = std::max(need, plan_segment(true, dense, batch, num_q_heads, num_kv_heads, prefix_tokens, sms).bytes +
-                              plan_segment(false, dense, batch, num_q_heads, num_kv_heads, cache_tokens, sms).bytes);
+  for (int format : {RA_CACHE_FP16, RA_CACHE_INT4})
+    need = std::max(need, plan_segment(true, format, batch, num_q_heads, num_kv_heads, prefix_tokens, sms).bytes +
+                              plan_segment(false, format, batch, num_q_heads, num_kv_heads, cache_tokens, sms).bytes);
   return 256 + need;
 }
 
@@ -255,9 +255,8 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;
     const int format = (i ? p->cache : p->prefix).format;
-    const bool dense = format <= RA_CACHE_BF16;
     const SegmentPlan s =
-        plan_segment(i == 0, dense, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
+        plan_segment(i == 0, format, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
     float* part_o = reinterpret_cast<float*>(at);
     float* part_ml = reinterpret_cast<float*>(at + s.ml_at);
     CombineSegment& c = cp.seg[i];
@@ -282,6 +281,9 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
       a.kmap = maps[0];
       a.vmap = maps[1];
       a.q = p->q;
+      a.k_scale = view[i].k_scale;
+      a.v_scale = view[i].v_scale;
+      a.scale_hstride = view[i].shstride;
       a.part_o = part_o;
       a.part_ml = part_ml;
       a.status = static_cast<unsigned*>(p->status);
@@ -293,7 +295,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
       a.group = cp.group;
       a.splits = s.splits;
       a.scale_log2e = p->sm_scale * kLog2e;
-      const cudaError_t e = launch_prefix_attend(a, bf16, stream);
+      const cudaError_t e = launch_prefix_attend(a, format, bf16, stream);
       if (e != cudaSuccess) return host_cuda_fail(e, "prefix_attend launch");
       continue;
     }

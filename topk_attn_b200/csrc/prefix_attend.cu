@@ -9,6 +9,8 @@
 // tiles; with one, they take the tiles in turn and leave a partial each.
 //   warp 0      TMA: K and V tiles of 32 KiB in one ring
 //   warps 1, 2  one thread of each issues a stream's MMAs; its commits release tiles and hand over S
+//   warps 12-15 for 8-bit caches: codes into fp16 or bf16 tiles, and the scales beside them; a token's K
+//               scale multiplies its column of S, its V scale its column of P, both in fp32
 //   warps 4-11  softmax: a thread owns one query (one TMEM lane), so maximum and sum need no exchange;
 //               P goes back into S's columns as the A operand of the second product
 // The maximum moves only when a score exceeds it by 2^4, and only then O is rescaled in TMEM; no wait
@@ -19,15 +21,28 @@
 
 namespace ra {
 
-constexpr int kPrefixStages = 5;
-constexpr int kPrefixThreads = 384;
-constexpr int kPrefixSoftRegs = 232, kPrefixOtherRegs = 40;   // 256 * 232 + 128 * 40 = 384 * 168
+// Dense tiles go straight from TMA to the MMAs.  8-bit codes pass a warpgroup that turns them into tiles
+// of fp16 or bf16, which hold every code exactly.
+__host__ __device__ constexpr int pf_stages(bool codes) { return codes ? 3 : 5; }      // of 32 KiB
+constexpr int kCodeStages = 3;                                     // of 16 KiB
+constexpr int kCodeBytes = kPrefixTile * 128;
+constexpr int kScaleTiles = 4;                                     // tiles whose scales are kept
+__host__ __device__ constexpr int pf_threads(bool codes) { return codes ? 512 : 384; }
+// registers: the softmax's 256 threads take over what the others give up
+//   dense: 256 * 232 + 128 * 40 = 384 * 168     codes: 256 * 184 + 128 * 40 + 128 * 104 = 512 * 128
+__host__ __device__ constexpr int pf_soft_regs(bool codes) { return codes ? 184 : 232; }
+constexpr int kPfOtherRegs = 40, kPfConvertRegs = 104;
 constexpr int kPrefixEarly = 64;                // tokens of P whose product starts while the rest is computed
 constexpr int kPrefixYield = 2;                 // quarter of P after which the other stream's turn begins
 constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f;
 
+struct PrefixScales {
+  float k[kScaleTiles][kPrefixTile];    // times the score scale
+  float v[kScaleTiles][kPrefixTile];
+  float top[kScaleTiles][4];            // largest |v| of 32 tokens
+};
 struct PrefixCtrl {
-  uint64_t full[kPrefixStages], empty[kPrefixStages];
+  uint64_t full[5], empty[5], code_full[kCodeStages], code_empty[kCodeStages];
   uint64_t q_full, s_full[2], p_full[2][2], o_full[2], turn[2], drain[2];
   uint32_t tmem;
   int timeout;
@@ -136,15 +151,49 @@ __device__ __forceinline__ uint32_t pf_pack(float lo, float hi) {
   return r;
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kPrefixThreads, 1)
+// Sixteen codes as eight pairs of fp16 or bf16.
+template <int FMT, bool BF16>
+__device__ __forceinline__ void pf_codes(const uint4& u, uint32_t (&r)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo, hi;
+    if (FMT == kCacheInt8) {
+      // a byte with its sign bit flipped in the low mantissa bits of 1024.0 is 1024 + 128 + code
+      const uint32_t x = w[i] ^ 0x80808080u, bias = 0x64806480u;
+      const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+      __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+      __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
+      lo = *reinterpret_cast<uint32_t*>(&ha);
+      hi = *reinterpret_cast<uint32_t*>(&hb);
+    } else {
+      asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+          : "=r"(lo), "=r"(hi)
+          : "r"(w[i]));
+    }
+    if (BF16) {
+      const float2 a = h2f2(lo), b = h2f2(hi);
+      lo = pf_pack<true>(a.x, a.y);
+      hi = pf_pack<true>(b.x, b.y);
+    }
+    r[2 * i] = lo;
+    r[2 * i + 1] = hi;
+  }
+}
+
+template <int FMT, bool BF16>
+__global__ void __launch_bounds__(pf_threads(FMT >= kCacheInt8), 1)
 prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
+  constexpr bool kCodes = FMT >= kCacheInt8;
+  constexpr int kPrefixStages = pf_stages(kCodes);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sm_q = smem;                                   // two query tiles
   unsigned char* sm_kv = smem + 2 * kPrefixTileBytes;           // ring of K and V tiles
-  PrefixCtrl* ctrl = reinterpret_cast<PrefixCtrl*>(sm_kv + kPrefixStages * kPrefixTileBytes);
+  unsigned char* sm_codes = sm_kv + kPrefixStages * kPrefixTileBytes;
+  PrefixScales* scales = reinterpret_cast<PrefixScales*>(sm_codes + (kCodes ? kCodeStages * kCodeBytes : 0));
+  PrefixCtrl* ctrl = reinterpret_cast<PrefixCtrl*>(reinterpret_cast<unsigned char*>(scales) + (kCodes ? sizeof(PrefixScales) : 0));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // ---- what this CTA works on; splits fastest, so that neighbours stream different tokens
@@ -162,8 +211,12 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     tma_prefetch_desc(&P.kmap);
     tma_prefetch_desc(&P.vmap);
     for (int s = 0; s < kPrefixStages; ++s) {
-      mbar_init(&ctrl->full[s], 1);
+      mbar_init(&ctrl->full[s], kCodes ? 128 : 1);
       mbar_init(&ctrl->empty[s], pair ? 2 : 1);
+    }
+    for (int s = 0; s < kCodeStages; ++s) {
+      mbar_init(&ctrl->code_full[s], 1);
+      mbar_init(&ctrl->code_empty[s], 128);
     }
     mbar_init(&ctrl->q_full, 256);
     for (int s = 0; s < 2; ++s) {
@@ -192,25 +245,28 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrefixOtherRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfOtherRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA
+      constexpr int kRing = kCodes ? kCodeStages : kPrefixStages;
+      constexpr int kBytes = kCodes ? kCodeBytes : kPrefixTileBytes;
+      uint64_t* full = kCodes ? ctrl->code_full : ctrl->full;
+      uint64_t* empty = kCodes ? ctrl->code_empty : ctrl->empty;
       int n = 0;
       for (; n < 2 * tiles; ++n) {
-        const int s = n % kPrefixStages;
-        if (!wait(&ctrl->empty[s], ((n / kPrefixStages) & 1) ^ 1)) break;
-        unsigned char* dst = sm_kv + s * kPrefixTileBytes;
+        const int s = n % kRing;
+        if (!wait(&empty[s], ((n / kRing) & 1) ^ 1)) break;
+        unsigned char* dst = (kCodes ? sm_codes : sm_kv) + s * kBytes;
         const CUtensorMap* map = (n & 1) ? &P.vmap : &P.kmap;
         const int tok = (tile0 + (n >> 1)) * kPrefixTile;
-        mbar_expect_tx(&ctrl->full[s], kPrefixTileBytes);
-        tma_load_4d(dst, map, &ctrl->full[s], 0, h, tok, 0);
-        tma_load_4d(dst + kPrefixHalf, map, &ctrl->full[s], 64, h, tok, 0);
+        mbar_expect_tx(&full[s], kBytes);
+        tma_load_4d(dst, map, &full[s], 0, h, tok, 0);
+        if (!kCodes) tma_load_4d(dst + kPrefixHalf, map, &full[s], 64, h, tok, 0);
       }
       // after a wait that ran out: no load may still be under way when the CTA ends
       if (n < 2 * tiles) {
         int own = 0;
-        for (int i = max(0, n - kPrefixStages); i < n; ++i)
-          mbar_wait(&ctrl->full[i % kPrefixStages], (i / kPrefixStages) & 1, &own);
+        for (int i = max(0, n - kRing); i < n; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1, &own);
       }
     } else if (warp == 1 || warp == 2) {
       // ---------------------------------------------------------------- MMA, stream warp - 1
@@ -244,8 +300,10 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       if (ok && j < tiles) scores(j);
       for (unsigned k = 0; ok && j < tiles; j += stride, ++k) {
         // the tiles first, so that the products follow one another once P is there
-        const bool more = j + stride < tiles;
-        ok = ready(2 * j + 1) && (!more || ready(2 * (j + stride)));
+        // (with three stages and one query tile the next K comes into the place of this V)
+        constexpr bool kDeepRing = kPrefixStages > 3;
+        const bool more = j + stride < tiles, early = kDeepRing || pair;
+        ok = ready(2 * j + 1) && (!more || !early || ready(2 * (j + stride)));
         const int s = (2 * j + 1) % kPrefixStages;
         const uint64_t b = v_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         ok = ok && wait(&ctrl->p_full[st][0], k & 1);
@@ -269,6 +327,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
           if (!more) tc_commit(&ctrl->o_full[st]);
         }
         __syncwarp();
+        if (more && !early && !(ok = ready(2 * (j + stride)))) break;
         if (more) scores(j + stride);
       }
       if (!ok) {   // no product may still be under way when TMEM is given back
@@ -279,8 +338,46 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       }
     }
     __syncwarp();
+  } else if (kCodes && warp >= 12) {
+    // ---------------------------------------------------------------- codes into tiles: a thread per token
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfConvertRegs));
+    const int t = tid - 384;
+    const long long at = (long long)h * P.scale_hstride + (long long)tile0 * kPrefixTile + t;
+    const int left = P.n_tokens - tile0 * kPrefixTile - t;       // tokens from mine on
+    float ks = left > 0 ? __ldg(P.k_scale + at) : 0.f, vs = left > 0 ? __ldg(P.v_scale + at) : 0.f;
+    for (int n = 0; n < 2 * tiles; ++n) {
+      const int j = n >> 1, s = n % kPrefixStages, c = n % kCodeStages, sj = j % kScaleTiles;
+      if (!__all_sync(0xffffffffu, wait(&ctrl->code_full[c], (n / kCodeStages) & 1) &&
+                                       wait(&ctrl->empty[s], ((n / kPrefixStages) & 1) ^ 1)))
+        break;
+      const uint32_t src = smem_u32(sm_codes) + c * kCodeBytes + t * 128;
+      unsigned char* dst = sm_kv + s * kPrefixTileBytes;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t r[8];
+        pf_codes<FMT, BF16>(lds128(src + ((i ^ (t & 7)) << 4)), r);
+        *reinterpret_cast<uint4*>(dst + swz128(t, 2 * i)) = make_uint4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<uint4*>(dst + swz128(t, 2 * i + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
+      }
+      // The slot of scales is free: of the four, tile j - 4 had it, and the loads whose stages the last two
+      // took, V of j - 2 and j - 3 among them, were released by products that follow their tiles' weights.
+      if (n & 1) {
+        scales->v[sj][t] = vs;
+        float top = fabsf(vs);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+        if (lane == 0) scales->top[sj][t >> 5] = top;
+        vs = left > (j + 1) * kPrefixTile ? __ldg(P.v_scale + at + (long long)(j + 1) * kPrefixTile) : 0.f;
+      } else {
+        scales->k[sj][t] = ks * P.scale_log2e;
+        ks = left > (j + 1) * kPrefixTile ? __ldg(P.k_scale + at + (long long)(j + 1) * kPrefixTile) : 0.f;
+      }
+      fence_proxy_async();
+      mbar_arrive(&ctrl->full[s]);
+      mbar_arrive(&ctrl->code_empty[c]);
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrefixSoftRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pf_soft_regs(kCodes)));
     // ---------------------------------------------------------------- queries into shared memory
     const int st = (warp >> 2) - 1;           // stream
     const int soft = tid - 128;
@@ -329,6 +426,20 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       tc_ld32(s + 64, tms + 64);
       tc_ld32(s + 96, tms + 96);
       tc_wait_ld();
+      const int sj = j % kScaleTiles;
+      if (kCodes) {
+        // the scales of both tiles were written before their tiles were handed over
+        ok = __all_sync(0xffffffffu, wait(&ctrl->full[(2 * j + 1) % kPrefixStages], ((2 * j + 1) / kPrefixStages) & 1));
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 128; c += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&scales->k[sj][c]);
+          s[c] = __float_as_uint(__uint_as_float(s[c]) * f.x);
+          s[c + 1] = __float_as_uint(__uint_as_float(s[c + 1]) * f.y);
+          s[c + 2] = __float_as_uint(__uint_as_float(s[c + 2]) * f.z);
+          s[c + 3] = __float_as_uint(__uint_as_float(s[c + 3]) * f.w);
+        }
+      }
       const int valid = P.n_tokens - (tile0 + j) * kPrefixTile;
       if (valid < kPrefixTile) {
 #pragma unroll
@@ -341,7 +452,15 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
         for (int d = 0; d < 4; ++d)
           mx4[d] = max3(mx4[d], __uint_as_float(s[c + d]), __uint_as_float(s[c + d + 4]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * P.scale_log2e;
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      if (kCodes) {
+        // the weights are multiplied by V's scales: the reference counts their largest in, and since sums
+        // and weights share the reference, it drops out in the end
+        const float top = fmaxf(fmaxf(scales->top[sj][0], scales->top[sj][1]), fmaxf(scales->top[sj][2], scales->top[sj][3]));
+        mx += fmaxf(-100.f, (float)((int)(__float_as_uint(top) >> 23) - 126));
+      } else {
+        mx *= P.scale_log2e;
+      }
       if (__any_sync(0xffffffffu, mx > m_ref + (kPfLazy + kPfLift))) {
         const float m_new = fmaxf(m_ref, mx - kPfLift), alpha = fast_exp2(m_ref - m_new);
         m_ref = m_new;
@@ -370,10 +489,16 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const int e = 32 * part + 2 * c;
-          float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, neg_m);
+          float2 x = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+          x = kCodes ? add2(x, neg_m) : fma2(x, scale2, neg_m);
           x.x = fast_exp2(x.x);
           x.y = fast_exp2(x.y);
           sum[c & 1] = add2(sum[c & 1], x);
+          if (kCodes) {
+            const float2 f = *reinterpret_cast<const float2*>(&scales->v[sj][e]);
+            x.x *= f.x;
+            x.y *= f.y;
+          }
           p[c] = pf_pack<BF16>(x.x, x.y);
         }
         tc_st16(tms + 16 * part, p);
@@ -433,16 +558,32 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   if (warp == 1) tc_free512(tmem);
 }
 
-cudaError_t launch_prefix_attend(const PrefixAttendParams& P, bool bf16, cudaStream_t stream) {
-  auto kern = bf16 ? prefix_attend_kernel<true> : prefix_attend_kernel<false>;
-  const size_t smem = (size_t)(2 + kPrefixStages) * kPrefixTileBytes + sizeof(PrefixCtrl) + 1024;
-  static std::atomic<unsigned long long> done[2];
-  const cudaError_t e = allow_smem(kern, smem, done[bf16]);
+namespace {
+
+template <int FMT, bool BF16>
+cudaError_t launch_one(const PrefixAttendParams& P, cudaStream_t stream) {
+  constexpr bool kCodes = FMT >= kCacheInt8;
+  auto kern = prefix_attend_kernel<FMT, BF16>;
+  const size_t smem = (size_t)(2 + pf_stages(kCodes)) * kPrefixTileBytes +
+                      (kCodes ? kCodeStages * kCodeBytes + sizeof(PrefixScales) : 0) + sizeof(PrefixCtrl) + 1024;
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return e;
   const int blocks = (P.query_tiles + 1) / 2 * P.hkv * P.splits;
   note_launch();
-  kern<<<blocks, kPrefixThreads, smem, stream>>>(P);
+  kern<<<blocks, pf_threads(kCodes), smem, stream>>>(P);
   return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_prefix_attend(const PrefixAttendParams& P, int format, bool bf16, cudaStream_t stream) {
+  switch (format) {
+    case kCacheFp16: return launch_one<kCacheFp16, false>(P, stream);
+    case kCacheBf16: return launch_one<kCacheBf16, true>(P, stream);
+    case kCacheInt8: return bf16 ? launch_one<kCacheInt8, true>(P, stream) : launch_one<kCacheInt8, false>(P, stream);
+    default: return bf16 ? launch_one<kCacheFp8, true>(P, stream) : launch_one<kCacheFp8, false>(P, stream);
+  }
 }
 
 }  // namespace ra

@@ -9,8 +9,11 @@ constexpr int kPrefixHalf = kPrefixTile * 128; // one swizzled [128 rows][128 by
 constexpr int kPrefixTileBytes = 2 * kPrefixHalf;
 
 struct PrefixAttendParams {
-  CUtensorMap kmap, vmap;   // 64-dim boxes of 128 tokens of one head
+  CUtensorMap kmap, vmap;   // boxes of 128 tokens of one head, 128 bytes wide
   const void* q;            // [batch, hq, 128]
+  const float* k_scale;     // of codes: [hkv][tokens], scale_hstride floats between heads
+  const float* v_scale;
+  long long scale_hstride;
   float* part_o;            // [(kv head, query tile)][2 splits][128][128] un-normalised sums
   float* part_ml;           // same, [2]: maximum (log2 domain), weight
   unsigned* status;
@@ -21,6 +24,7 @@ struct PrefixAttendParams {
   float scale_log2e;
 };
 
-cudaError_t launch_prefix_attend(const PrefixAttendParams& P, bool bf16, cudaStream_t stream);
+// format: not int4, whose scales lie along the dims and cannot be applied to S
+cudaError_t launch_prefix_attend(const PrefixAttendParams& P, int format, bool bf16, cudaStream_t stream);
 
 }  // namespace ra
