@@ -82,6 +82,15 @@ def test_prefix_and_own_caches(B, Hq, Hkv, Np, N, kind, dtype):
     check(q, prefix, own, kind, lens)
 
 
+@pytest.mark.parametrize("kind,dtype", [("", torch.float16), ("", torch.bfloat16), ("int8", torch.float16),
+                                        ("fp8", torch.bfloat16), ("int4", torch.float16)])
+@pytest.mark.parametrize("B,Np", [(24, 123457), (131, 98304)])
+def test_many_tiles_for_each_part(kind, dtype, B, Np):
+    """One kv head, so that every CTA walks a long run of tiles: one and two tiles of queries."""
+    q, prefix, own = make(B, 1, 1, Np, 2, kind, dtype, 5)
+    check(q, prefix, own, kind)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_prefix_alone_and_a_shared_quantised_cache(kind):
     from topk_attn_b200 import ops

@@ -23,7 +23,8 @@ namespace ra {
 
 // Dense tiles go straight from TMA to the MMAs.  8-bit codes pass a warpgroup that turns them into tiles
 // of fp16 or bf16, which hold every code exactly.
-__host__ __device__ constexpr int pf_stages(bool codes) { return codes ? 3 : 5; }      // of 32 KiB
+__host__ __device__ constexpr int pf_stages(bool codes) { return codes ? 3 : 5; }      // of 32 KiB, one more where
+                                                                   // only one query tile is held
 constexpr int kCodeStages = 3;                                     // of 16 KiB
 constexpr int kCodeBytes = kPrefixTile * 128;
 constexpr int kScaleTiles = 4;                                     // tiles whose scales are kept
@@ -42,7 +43,7 @@ struct PrefixScales {
   float top[kScaleTiles][4];            // largest |v| of 32 tokens
 };
 struct PrefixCtrl {
-  uint64_t full[5], empty[5], code_full[kCodeStages], code_empty[kCodeStages];
+  uint64_t full[6], empty[6], code_full[kCodeStages], code_empty[kCodeStages], scales_full[kScaleTiles];
   uint64_t q_full, s_full[2], p_full[2][2], o_full[2], turn[2], drain[2];
   uint32_t tmem;
   int timeout;
@@ -124,6 +125,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -185,13 +193,11 @@ template <int FMT, bool BF16>
 __global__ void __launch_bounds__(pf_threads(FMT >= kCacheInt8), 1)
 prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   constexpr bool kCodes = FMT >= kCacheInt8;
-  constexpr int kPrefixStages = pf_stages(kCodes);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sm_q = smem;                                   // two query tiles
-  unsigned char* sm_kv = smem + 2 * kPrefixTileBytes;           // ring of K and V tiles
-  unsigned char* sm_codes = sm_kv + kPrefixStages * kPrefixTileBytes;
+  unsigned char* sm_codes = smem + (2 + pf_stages(kCodes)) * kPrefixTileBytes;
   PrefixScales* scales = reinterpret_cast<PrefixScales*>(sm_codes + (kCodes ? kCodeStages * kCodeBytes : 0));
   PrefixCtrl* ctrl = reinterpret_cast<PrefixCtrl*>(reinterpret_cast<unsigned char*>(scales) + (kCodes ? sizeof(PrefixScales) : 0));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -200,17 +206,23 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   const int split = blockIdx.x % P.splits, rest = blockIdx.x / P.splits;
   const int h = rest % P.hkv, qt0 = 2 * (rest / P.hkv);
   const bool pair = qt0 + 1 < P.query_tiles;
+  // ring of K and V tiles; the second query tile's place is one of them where there is none
+  unsigned char* sm_kv = smem + (pair ? 2 : 1) * kPrefixTileBytes;
+  const int stages = pf_stages(kCodes) + (pair ? 0 : 1);
   const int all_tiles = ceil_div(P.n_tokens, kPrefixTile);
   const int tile0 = (int)((long long)all_tiles * split / P.splits);
   const int tiles = (int)((long long)all_tiles * (split + 1) / P.splits) - tile0;
-  // stream s walks the tiles s, s + 2, .. of one query tile, or all of them for query tile s; tile j's K
-  // is load 2 j of the ring, its V load 2 j + 1
+  // stream s walks the tiles s, s + 2, .. of one query tile, or all of them for query tile s.  Tiles are
+  // loaded in the order of their first use: K of the first `stride` tiles, then V of tile j and K of
+  // tile j + stride for each j, as far as there are any.
   const int stride = pair ? 1 : 2;
+  auto k_load = [&](int j) { return j + max(0, j - stride + 1); };
+  auto v_load = [&](int j) { return j + min(tiles, j + stride); };
 
   if (tid == 0) {
     tma_prefetch_desc(&P.kmap);
     tma_prefetch_desc(&P.vmap);
-    for (int s = 0; s < kPrefixStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&ctrl->full[s], kCodes ? 128 : 1);
       mbar_init(&ctrl->empty[s], pair ? 2 : 1);
     }
@@ -218,6 +230,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       mbar_init(&ctrl->code_full[s], 1);
       mbar_init(&ctrl->code_empty[s], 128);
     }
+    for (int s = 0; s < kScaleTiles; ++s) mbar_init(&ctrl->scales_full[s], 128);
     mbar_init(&ctrl->q_full, 256);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctrl->s_full[s], 1);
@@ -248,25 +261,31 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfOtherRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA
-      constexpr int kRing = kCodes ? kCodeStages : kPrefixStages;
+      const int ring = kCodes ? kCodeStages : stages;
       constexpr int kBytes = kCodes ? kCodeBytes : kPrefixTileBytes;
       uint64_t* full = kCodes ? ctrl->code_full : ctrl->full;
       uint64_t* empty = kCodes ? ctrl->code_empty : ctrl->empty;
       int n = 0;
-      for (; n < 2 * tiles; ++n) {
-        const int s = n % kRing;
-        if (!wait(&empty[s], ((n / kRing) & 1) ^ 1)) break;
+      auto load = [&](const CUtensorMap* map, int tile) {
+        const int s = n % ring;
+        if (!wait(&empty[s], ((n / ring) & 1) ^ 1)) return false;
         unsigned char* dst = (kCodes ? sm_codes : sm_kv) + s * kBytes;
-        const CUtensorMap* map = (n & 1) ? &P.vmap : &P.kmap;
-        const int tok = (tile0 + (n >> 1)) * kPrefixTile;
+        const int tok = (tile0 + tile) * kPrefixTile;
         mbar_expect_tx(&full[s], kBytes);
         tma_load_4d(dst, map, &full[s], 0, h, tok, 0);
         if (!kCodes) tma_load_4d(dst + kPrefixHalf, map, &full[s], 64, h, tok, 0);
+        ++n;
+        return true;
+      };
+      bool ok = true;
+      for (int j = -stride; ok && j < tiles; ++j) {
+        if (j >= 0) ok = load(&P.vmap, j);
+        if (ok && j + stride < tiles) ok = load(&P.kmap, j + stride);
       }
       // after a wait that ran out: no load may still be under way when the CTA ends
-      if (n < 2 * tiles) {
+      if (!ok) {
         int own = 0;
-        for (int i = max(0, n - kRing); i < n; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1, &own);
+        for (int i = max(0, n - ring); i < n; ++i) mbar_wait(&full[i % ring], (i / ring) & 1, &own);
       }
     } else if (warp == 1 || warp == 2) {
       // ---------------------------------------------------------------- MMA, stream warp - 1
@@ -279,9 +298,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       const uint64_t q_desc = tc_desc(smem_u32(sm_q) + (pair ? st * kPrefixTileBytes : 0), 16, 1024);
       const uint64_t k_desc = tc_desc(smem_u32(sm_kv), 16, 1024);
       const uint64_t v_desc = tc_desc(smem_u32(sm_kv), kPrefixHalf, 1024);
-      auto ready = [&](int n) { return wait(&ctrl->full[n % kPrefixStages], (n / kPrefixStages) & 1); };
+      auto ready = [&](int n) { return wait(&ctrl->full[n % stages], (n / stages) & 1); };
       auto scores = [&](int j) {
-        const int s = 2 * j % kPrefixStages;
+        const int s = k_load(j) % stages;
         const uint64_t b = k_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         tc_fence_after();
         if (elect_one()) {
@@ -296,15 +315,13 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         __syncwarp();
       };
       int j = pair ? 0 : st;
-      bool ok = wait(&ctrl->q_full, 0) && (j >= tiles || ready(2 * j));
+      bool ok = wait(&ctrl->q_full, 0) && (j >= tiles || ready(k_load(j)));
       if (ok && j < tiles) scores(j);
       for (unsigned k = 0; ok && j < tiles; j += stride, ++k) {
         // the tiles first, so that the products follow one another once P is there
-        // (with three stages and one query tile the next K comes into the place of this V)
-        constexpr bool kDeepRing = kPrefixStages > 3;
-        const bool more = j + stride < tiles, early = kDeepRing || pair;
-        ok = ready(2 * j + 1) && (!more || !early || ready(2 * (j + stride)));
-        const int s = (2 * j + 1) % kPrefixStages;
+        const bool more = j + stride < tiles;
+        ok = ready(v_load(j)) && (!more || ready(k_load(j + stride)));
+        const int s = v_load(j) % stages;
         const uint64_t b = v_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         ok = ok && wait(&ctrl->p_full[st][0], k & 1);
         if (!ok) break;
@@ -327,7 +344,6 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
           if (!more) tc_commit(&ctrl->o_full[st]);
         }
         __syncwarp();
-        if (more && !early && !(ok = ready(2 * (j + stride)))) break;
         if (more) scores(j + stride);
       }
       if (!ok) {   // no product may still be under way when TMEM is given back
@@ -345,36 +361,55 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     const long long at = (long long)h * P.scale_hstride + (long long)tile0 * kPrefixTile + t;
     const int left = P.n_tokens - tile0 * kPrefixTile - t;       // tokens from mine on
     float ks = left > 0 ? __ldg(P.k_scale + at) : 0.f, vs = left > 0 ? __ldg(P.v_scale + at) : 0.f;
-    for (int n = 0; n < 2 * tiles; ++n) {
-      const int j = n >> 1, s = n % kPrefixStages, c = n % kCodeStages, sj = j % kScaleTiles;
-      if (!__all_sync(0xffffffffu, wait(&ctrl->code_full[c], (n / kCodeStages) & 1) &&
-                                       wait(&ctrl->empty[s], ((n / kPrefixStages) & 1) ^ 1)))
-        break;
-      const uint32_t src = smem_u32(sm_codes) + c * kCodeBytes + t * 128;
-      unsigned char* dst = sm_kv + s * kPrefixTileBytes;
+    // V of tile j and K of tile j + stride together: one round of waits, one fence
+    for (int j = -stride; j < tiles; ++j) {
+      const int jk = j + stride, sj = jk % kScaleTiles;
+      const bool has[2] = {j >= 0, jk < tiles};
+      const int load[2] = {v_load(j), k_load(jk)};
+      bool go = true;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t r[8];
-        pf_codes<FMT, BF16>(lds128(src + ((i ^ (t & 7)) << 4)), r);
-        *reinterpret_cast<uint4*>(dst + swz128(t, 2 * i)) = make_uint4(r[0], r[1], r[2], r[3]);
-        *reinterpret_cast<uint4*>(dst + swz128(t, 2 * i + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
+      for (int i = 0; i < 2; ++i)
+        if (has[i])
+          go = go && wait(&ctrl->code_full[load[i] % kCodeStages], (load[i] / kCodeStages) & 1) &&
+               wait(&ctrl->empty[load[i] % stages], ((load[i] / stages) & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, go)) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!has[i]) continue;
+        const int c = load[i] % kCodeStages;
+        const uint32_t src = smem_u32(sm_codes) + c * kCodeBytes + t * 128;
+        unsigned char* dst = sm_kv + (load[i] % stages) * kPrefixTileBytes;
+        uint4 u[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) u[d] = lds128(src + ((d ^ (t & 7)) << 4));
+        mbar_arrive(&ctrl->code_empty[c]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          uint32_t r[8];
+          pf_codes<FMT, BF16>(u[d], r);
+          *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d)) = make_uint4(r[0], r[1], r[2], r[3]);
+          *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
+        }
       }
-      // The slot of scales is free: of the four, tile j - 4 had it, and the loads whose stages the last two
-      // took, V of j - 2 and j - 3 among them, were released by products that follow their tiles' weights.
-      if (n & 1) {
+      fence_proxy_async();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (has[i]) mbar_arrive(&ctrl->full[load[i] % stages]);
+      if (has[1]) {
+        // both scales of tile jk.  Their slot of four was tile jk - 4's, whose weights are done: the stage
+        // of V of jk - stride, or of this K, was released by the product of a tile of jk - 4 or later of
+        // the same stream (of both, where both walk all tiles), and products follow their weights.
+        scales->k[sj][t] = ks * P.scale_log2e;
         scales->v[sj][t] = vs;
         float top = fabsf(vs);
 #pragma unroll
         for (int i = 16; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
         if (lane == 0) scales->top[sj][t >> 5] = top;
-        vs = left > (j + 1) * kPrefixTile ? __ldg(P.v_scale + at + (long long)(j + 1) * kPrefixTile) : 0.f;
-      } else {
-        scales->k[sj][t] = ks * P.scale_log2e;
-        ks = left > (j + 1) * kPrefixTile ? __ldg(P.k_scale + at + (long long)(j + 1) * kPrefixTile) : 0.f;
+        mbar_arrive(&ctrl->scales_full[sj]);
+        const bool next = left > (jk + 1) * kPrefixTile;
+        ks = next ? __ldg(P.k_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
+        vs = next ? __ldg(P.v_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
       }
-      fence_proxy_async();
-      mbar_arrive(&ctrl->full[s]);
-      mbar_arrive(&ctrl->code_empty[c]);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pf_soft_regs(kCodes)));
@@ -428,16 +463,17 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       tc_wait_ld();
       const int sj = j % kScaleTiles;
       if (kCodes) {
-        // the scales of both tiles were written before their tiles were handed over
-        ok = __all_sync(0xffffffffu, wait(&ctrl->full[(2 * j + 1) % kPrefixStages], ((2 * j + 1) / kPrefixStages) & 1));
+        ok = __all_sync(0xffffffffu, wait(&ctrl->scales_full[sj], (j / kScaleTiles) & 1));
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < 128; c += 4) {
           const float4 f = *reinterpret_cast<const float4*>(&scales->k[sj][c]);
-          s[c] = __float_as_uint(__uint_as_float(s[c]) * f.x);
-          s[c + 1] = __float_as_uint(__uint_as_float(s[c + 1]) * f.y);
-          s[c + 2] = __float_as_uint(__uint_as_float(s[c + 2]) * f.z);
-          s[c + 3] = __float_as_uint(__uint_as_float(s[c + 3]) * f.w);
+          const float2 a = mul2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(f.x, f.y));
+          const float2 b = mul2(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), make_float2(f.z, f.w));
+          s[c] = __float_as_uint(a.x);
+          s[c + 1] = __float_as_uint(a.y);
+          s[c + 2] = __float_as_uint(b.x);
+          s[c + 3] = __float_as_uint(b.y);
         }
       }
       const int valid = P.n_tokens - (tile0 + j) * kPrefixTile;
@@ -487,19 +523,20 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       for (int part = 0; part < 4; ++part) {
         uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
+        for (int c = 0; c < 16; c += 2) {
           const int e = 32 * part + 2 * c;
-          float2 x = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-          x = kCodes ? add2(x, neg_m) : fma2(x, scale2, neg_m);
-          x.x = fast_exp2(x.x);
-          x.y = fast_exp2(x.y);
-          sum[c & 1] = add2(sum[c & 1], x);
-          if (kCodes) {
-            const float2 f = *reinterpret_cast<const float2*>(&scales->v[sj][e]);
-            x.x *= f.x;
-            x.y *= f.y;
+          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (kCodes) f = *reinterpret_cast<const float4*>(&scales->v[sj][e]);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            float2 x = make_float2(__uint_as_float(s[e + 2 * d]), __uint_as_float(s[e + 2 * d + 1]));
+            x = kCodes ? add2(x, neg_m) : fma2(x, scale2, neg_m);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
+            sum[d] = add2(sum[d], x);
+            if (kCodes) x = mul2(x, d ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+            p[c + d] = pf_pack<BF16>(x.x, x.y);
           }
-          p[c] = pf_pack<BF16>(x.x, x.y);
         }
         tc_st16(tms + 16 * part, p);
         if (part == kPrefixYield) mbar_arrive(&ctrl->turn[st ^ 1]);
@@ -520,10 +557,10 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       __syncwarp();
       tc_fence_after();
     }
-    // 32 rows x 32 dims at a time through shared memory, so that rows leave in whole lines.  The query
-    // tile is free: with one tile the other's place is used, where no product reads.
-    const uint32_t buf = smem_u32(sm_q) + (pair ? st * kPrefixTileBytes + (warp & 3) * 4096
-                                                : kPrefixTileBytes + (warp - 4) * 4096);
+    // 32 rows x 32 dims at a time through shared memory, so that rows leave in whole lines: in the stream's
+    // query tile, or in the one that both read once both are done
+    if (!pair) asm volatile("bar.sync 2, 256;" ::: "memory");
+    const uint32_t buf = smem_u32(sm_q) + (pair ? st * kPrefixTileBytes + (warp & 3) * 4096 : (warp - 4) * 4096);
     const int live = P.queries - qt * kPrefixTile - row0;  // rows of mine that are queries
     float* out = P.part_o + (slot * kPrefixTile + row0) * kHeadDim;
 #pragma unroll 1
