@@ -98,9 +98,14 @@ __device__ __forceinline__ void codes_of(uint32_t w, uint32_t& first, uint32_t& 
         : "r"(w));
   }
 }
-// nibbles (i, i + 4) of a word, which hold code + 8
+// Nibbles (i, i + 4) of a word hold code + 8.  raw: as they are, an fp16 subnormal of (code + 8) 2^-24,
+// the odd ones 16 times that; otherwise exact codes, the odd ones 16 times.
+__device__ __forceinline__ uint32_t nibbles_raw(uint32_t w, int i) {
+  return (i < 2 ? w : w >> 8) & ((i & 1) ? 0x00f000f0u : 0x000f000fu);
+}
 __device__ __forceinline__ uint32_t nibbles_of(uint32_t w, int i) {
-  return hsub2_bits(((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, 0x64086408u);
+  return (i & 1) ? hsub2_bits(nibbles_raw(w, i) | 0x64006400u, 0x64806480u)
+                 : hsub2_bits(nibbles_raw(w, i) | 0x64006400u, 0x64086408u);
 }
 
 // My part of one work row: tiles [first, first + count) of (cache b, kv head h, query tile qt), and the
@@ -332,6 +337,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     }
     // B fragments of Q^T: column g is query q0 + 8 nq + g; the dims of lane t in the order K's lanes hold them
     uint32_t qb[NQ][8][2];
+    float k_off[NQ][FMT == kCacheInt4 ? 4 : 1][2];
     float fac[NQ][2];      // what turns a raw score of my two columns into the log2 domain
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
@@ -384,9 +390,24 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
           constexpr int i1 = FMT == kCacheInt4 ? 4 : FMT == kCacheInt8 ? 2 : 1;
           constexpr int i2 = FMT == kCacheFp8 ? 2 : 1;
           qb[nq][kk][0] = pack_pair<false>(y[0] * down, y[i1] * down);
-          qb[nq][kk][1] = pack_pair<false>(y[i2] * down, y[i2 + i1] * down);
+          constexpr float kOdd = FMT == kCacheInt4 ? 0.0625f : 1.f;     // K's odd nibbles come 16 times as large
+          qb[nq][kk][1] = pack_pair<false>(y[i2] * down * kOdd, y[i2 + i1] * down * kOdd);
         }
-        const float up = __uint_as_float(top) * P.scale_log2e;
+        if (FMT == kCacheInt4) {
+          // sum over a group of q (code + 8) less 8 times the sum of q: what the accumulators start from
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += x[8 * j + i];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= down * (-8.f / 16777216.f);
+            k_off[nq][j][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+            k_off[nq][j][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+          }
+        }
+        const float up = __uint_as_float(top) * P.scale_log2e * (FMT == kCacheInt4 ? 16777216.f : 1.f);
         fac[nq][0] = __shfl_sync(0xffffffffu, up, 8 * t);
         fac[nq][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
       }
@@ -454,11 +475,14 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
             const uint32_t wb = lds32(kbase + tb * 64 + ((j ^ ((tb >> 1) & 3)) << 4) + 4 * t);
             float part[NQ][4];
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) part[nq][0] = part[nq][1] = part[nq][2] = part[nq][3] = 0.f;
+            for (int nq = 0; nq < NQ; ++nq) {
+              part[nq][0] = part[nq][2] = k_off[nq][FMT == kCacheInt4 ? j : 0][0];
+              part[nq][1] = part[nq][3] = k_off[nq][FMT == kCacheInt4 ? j : 0][1];
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t a[4] = {nibbles_of(wa, 2 * i), nibbles_of(wb, 2 * i), nibbles_of(wa, 2 * i + 1),
-                                     nibbles_of(wb, 2 * i + 1)};
+              const uint32_t a[4] = {nibbles_raw(wa, 2 * i), nibbles_raw(wb, 2 * i), nibbles_raw(wa, 2 * i + 1),
+                                     nibbles_raw(wb, 2 * i + 1)};
 #pragma unroll
               for (int nq = 0; nq < NQ; ++nq) mma_16816(part[nq], a, qb[nq][2 * j + i][0], qb[nq][2 * j + i][1]);
             }
@@ -706,7 +730,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
               float* p = dst + (2 * t + i) * kMergePitch;
               if (FMT == kCacheInt4) {
                 *reinterpret_cast<float2*>(p + 32 * (m4 >> 1) + 4 * g + 2 * (m4 & 1)) =
-                    make_float2(o[nq][mt][i] * f[i], o[nq][mt][i + 2] * f[i]);
+                    make_float2(o[nq][mt][i] * f[i], o[nq][mt][i + 2] * (f[i] * 0.0625f));   // odd nibble
               } else {
                 p[16 * m4 + g] = o[nq][mt][i] * f[i];
                 p[16 * m4 + g + 8] = o[nq][mt][i + 2] * f[i];
