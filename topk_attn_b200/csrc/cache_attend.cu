@@ -61,6 +61,12 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// asynchronous copy of 4 or 16 bytes, or as many zeros
+template <int BYTES>
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(live ? BYTES : 0)
+               : "memory");
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   uint32_t r;
@@ -124,13 +130,16 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
   constexpr int kHalf = kAttendTile * 128;          // one swizzled [64 tokens][128 bytes] block
   constexpr int kKBytes = kAttendTile * cache_row_bytes(FMT);
   constexpr int kStage = 2 * kKBytes;
+  constexpr int kNS = kDense ? 1 : cache_row_scales(FMT);
+  constexpr int kScaleFloats = attend_scale_floats(FMT);
   constexpr int QT = 8 * NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const AttendSegment& G = P.seg;
   const int S = G.nstages;
-  float* sm_o = reinterpret_cast<float*>(smem + (size_t)S * kStage);   // [4 warps][8 queries][68]
+  float* sm_sc = reinterpret_cast<float*>(smem + (size_t)S * kStage);  // [stages][K, V][64 tokens][scales]
+  float* sm_o = sm_sc + S * kScaleFloats;                               // [4 warps][8 queries][68]
   AttendCtrl<NQ>* ctrl = reinterpret_cast<AttendCtrl<NQ>*>(reinterpret_cast<unsigned char*>(sm_o) + kMergeBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per_cache = P.hkv * G.query_tiles;
@@ -139,7 +148,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     tma_prefetch_desc(&G.kmap);
     tma_prefetch_desc(&G.vmap);
     for (int s = 0; s < S; ++s) {
-      mbar_init(&ctrl->full[s], 1);
+      mbar_init(&ctrl->full[s], kDense ? 1 : 33);      // the TMA's arrival and each lane's scales
       mbar_init(&ctrl->empty[s], kAttendWarps);
     }
     ctrl->timeout = 0;
@@ -245,14 +254,19 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 
   if (warp == kAttendWarps) {
     // ---------------------------------------------------------------- producer warp
-    if (lane == 0) {
-      int s = 0;
-      unsigned parity = 1;          // of the phase before the first: an unused stage is free
-      for (;;) {
-        for (int i = 0; i < row.count; ++i) {
-          if (!mbar_wait(&ctrl->empty[s], parity, &ctrl->timeout)) atomicOr(P.status, kStatusTimeout);
-          unsigned char* dst = smem + (size_t)s * kStage;
-          const int tok = (row.first + i) * kAttendTile;
+    // lane 0 starts the TMA copies; all lanes fetch the scales, which would otherwise come one tile
+    // ahead at most and pay the memory's loaded latency for every tile
+    int s = 0, issued = 0;
+    unsigned parity = 1;          // of the phase before the first: an unused stage is free
+    bool ok = true;
+    while (ok) {
+      const long long sbase = (long long)row.b * G.cache.sbstride + (long long)row.h * G.cache.shstride;
+      for (int i = 0; ok && i < row.count; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&ctrl->empty[s], parity, &ctrl->timeout));
+        if (!ok) break;
+        unsigned char* dst = smem + (size_t)s * kStage;
+        const int tok = (row.first + i) * kAttendTile;
+        if (lane == 0) {
           mbar_expect_tx(&ctrl->full[s], kStage);
           if (kDense) {
             tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, row.h, tok, row.b);
@@ -263,16 +277,37 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
             tma_load_4d(dst, &G.kmap, &ctrl->full[s], 0, row.h, tok, row.b);
             tma_load_4d(dst + kKBytes, &G.vmap, &ctrl->full[s], 0, row.h, tok, row.b);
           }
-          if (++s == S) {
-            s = 0;
-            parity ^= 1;
-          }
         }
-        left -= row.units;
-        if (left <= 0) break;
-        row = row_behind(row, left);
+        if (!kDense) {
+          const uint32_t sc = smem_u32(sm_sc + s * kScaleFloats);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = lane + 32 * (j & 1);      // token of the tile; K for j < 2, then V
+            const bool live = tok + t < row.len;    // zeros for the others
+            const float* src = ((j >> 1) ? G.cache.v_scale : G.cache.k_scale) + (live ? sbase + (long long)(tok + t) * kNS : 0);
+            cp_async_zfill<4 * kNS>(sc + ((j >> 1) * kAttendTile + t) * 4 * kNS, src, live);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctrl->full[s])) : "memory");
+        }
+        ++issued;
+        if (++s == S) {
+          s = 0;
+          parity ^= 1;
+        }
       }
+      left -= row.units;
+      if (left <= 0) break;
+      row = row_behind(row, left);
     }
+    if (!ok) {
+      // a wait ran out: the consumers carry on, but no copy may still be under way when the CTA ends
+      if (lane == 0) atomicOr(P.status, kStatusTimeout);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      int own = 0;
+      for (int i = max(0, issued - S); i < issued; ++i)
+        mbar_wait(&ctrl->full[i % S], (unsigned)((i / S) & 1), &own, kWaitLimitNs / 4);
+    }
+    if (P.after) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
 
@@ -281,35 +316,6 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
   const int r0 = warp * 16;
   const uint32_t stage0 = smem_u32(smem);
   const int mi = lane >> 3, lr = lane & 7;
-  // scales of the next tile, fetched one tile ahead: tokens g and g + 8 of my 16
-  constexpr int kNS = kDense ? 1 : cache_row_scales(FMT);
-  float ks_next[2][kNS], vs_next[2][kNS];
-  auto fetch_scales = [&](const float* kp, const float* vp, int tok, int len) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool live = tok + 8 * i < len;
-      if (kNS == 4) {
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = live ? __ldg(reinterpret_cast<const float4*>(kp) + 8 * i) : z;
-        const float4 b = live ? __ldg(reinterpret_cast<const float4*>(vp) + 8 * i) : z;
-        ks_next[i][0] = a.x; ks_next[i][kNS > 1 ? 1 : 0] = a.y; ks_next[i][kNS > 2 ? 2 : 0] = a.z; ks_next[i][kNS - 1] = a.w;
-        vs_next[i][0] = b.x; vs_next[i][kNS > 1 ? 1 : 0] = b.y; vs_next[i][kNS > 2 ? 2 : 0] = b.z; vs_next[i][kNS - 1] = b.w;
-      } else {
-        ks_next[i][0] = live ? __ldg(kp + 8 * i) : 0.f;
-        vs_next[i][0] = live ? __ldg(vp + 8 * i) : 0.f;
-      }
-    }
-  };
-  // where this lane's scales of a row's tile begin
-  auto scale_offset = [&](const AttendRow& r, int tile) {
-    return (long long)r.b * G.cache.sbstride + (long long)r.h * G.cache.shstride +
-           (long long)(tile * kAttendTile + r0 + g) * kNS;
-  };
-  if (!kDense) {
-    const long long at = scale_offset(row, row.first);
-    fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, row.first * kAttendTile + r0 + g, row.len);
-  }
-
   int s = 0;
   unsigned parity = 0;
   for (;;) {
@@ -320,21 +326,10 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     if (row.count == 0) {             // none of its tiles, only of the units before them
       if (left <= 0) break;
       row = behind;
-      if (!kDense) {
-        const long long at = scale_offset(row, 0);
-        fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, r0 + g, row.len);
-      }
       continue;
     }
     const int b = row.b, h = row.h, q0 = row.qt * QT, len = row.len;
     const long long slot = (long long)b * per_cache + row.inner + blockIdx.x;
-    const float* kp = nullptr;
-    const float* vp = nullptr;
-    if (!kDense) {
-      const long long at = scale_offset(row, row.first);
-      kp = G.cache.k_scale + at;
-      vp = G.cache.v_scale + at;
-    }
     // B fragments of Q^T: column g is query q0 + 8 nq + g; the dims of lane t in the order K's lanes hold them
     uint32_t qb[NQ][8][2];
     float k_off[NQ][FMT == kCacheInt4 ? 4 : 1][2];
@@ -425,30 +420,28 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 
     for (int i_tile = 0; i_tile < row.count; ++i_tile) {
       const int tok0 = (row.first + i_tile) * kAttendTile + r0;     // my 16 tokens
-      float ks[2][kNS], vs[2][kNS];
-      if (!kDense) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < kNS; ++j) {
-            ks[i][j] = ks_next[i][j];
-            vs[i][j] = vs_next[i][j];
-          }
-        if (i_tile + 1 < row.count) {
-          kp += kAttendTile * kNS;
-          vp += kAttendTile * kNS;
-          fetch_scales(kp, vp, tok0 + kAttendTile + g, len);
-        } else if (left > 0) {
-          const long long at = scale_offset(behind, 0);
-          fetch_scales(G.cache.k_scale + at, G.cache.v_scale + at, r0 + g, behind.len);
-        }
-      }
       if (!mbar_wait(&ctrl->full[s], parity, &ctrl->timeout)) {
         if (lane == 0) atomicOr(P.status, kStatusTimeout);
       }
       if (tok0 < len) {
         const uint32_t kbase = stage0 + (uint32_t)s * kStage, vbase = kbase + kKBytes;
         const bool tail = tok0 + 16 > len;
+        float ks[2][kNS], vs[2][kNS];     // of tokens g and g + 8 of my 16
+        if (!kDense) {
+          const float* sc = sm_sc + s * kScaleFloats + (r0 + g) * kNS;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (kNS == 4) {
+              const float4 a = *reinterpret_cast<const float4*>(sc + 8 * i * kNS);
+              const float4 c = *reinterpret_cast<const float4*>(sc + (kAttendTile + 8 * i) * kNS);
+              ks[i][0] = a.x; ks[i][kNS > 1 ? 1 : 0] = a.y; ks[i][kNS > 2 ? 2 : 0] = a.z; ks[i][kNS - 1] = a.w;
+              vs[i][0] = c.x; vs[i][kNS > 1 ? 1 : 0] = c.y; vs[i][kNS > 2 ? 2 : 0] = c.z; vs[i][kNS - 1] = c.w;
+            } else {
+              ks[i][0] = sc[8 * i];
+              vs[i][0] = sc[kAttendTile + 8 * i];
+            }
+          }
+        }
         // ---- S^T = K Q^T
         float x[NQ][4];
 #pragma unroll
@@ -844,7 +837,7 @@ int stage_bytes(int format) { return 2 * kAttendTile * cache_row_bytes(format); 
 
 // Three CTAs of a multiprocessor share 228 KiB, or two.
 int cache_attend_stages(int format, int nq) {
-  const int n = (nq == 1 ? 65536 : 98304) / stage_bytes(format);
+  const int n = (nq == 1 ? 65536 : 98304) / (stage_bytes(format) + 4 * attend_scale_floats(format));
   return n < kAttendMaxStages ? n : kAttendMaxStages;
 }
 
@@ -853,7 +846,7 @@ namespace {
 template <int FMT, bool BF16, int NQ>
 cudaError_t launch_one(const CacheAttendParams& P, cudaStream_t stream) {
   auto kern = cache_attend_kernel<FMT, BF16, NQ>;
-  const size_t smem = (size_t)P.seg.nstages * stage_bytes(FMT) + kMergeBytes + sizeof(AttendCtrl<NQ>) + 1024;
+  const size_t smem = (size_t)P.seg.nstages * (stage_bytes(FMT) + 4 * attend_scale_floats(FMT)) + kMergeBytes + sizeof(AttendCtrl<NQ>) + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return e;

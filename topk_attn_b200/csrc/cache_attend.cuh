@@ -8,6 +8,8 @@ constexpr int kAttendTile = 64;                // tokens per pipeline stage
 constexpr int kAttendWarps = 4;                // consumer warps, 16 tokens of a tile each
 constexpr int kAttendThreads = 32 * (kAttendWarps + 1);
 constexpr int kAttendMaxStages = 8;
+// scales of a tile, K's and then V's
+__host__ __device__ constexpr int attend_scale_floats(int format) { return 2 * kAttendTile * cache_row_scales(format); }
 // What beginning and ending a work row costs, in tiles: loading its queries, merging the warps' sums.
 constexpr int kAttendRowUnits = 2;
 // CTAs per multiprocessor: three with 8 query columns (128 registers a thread), two with 16
