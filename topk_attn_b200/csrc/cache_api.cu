@@ -145,7 +145,17 @@ int prefix_splits(int blocks, int tiles, int sms) {
   return best;
 }
 
-SegmentPlan plan_segment(bool prefix, int format, int batch, int hq, int hkv, int tokens, int sms) {
+// Where every cache is equally long and is held in 8 bits, the grid is a multiple of the rows, so that the
+// heads, whose 128-byte rows lie side by side in memory, are walked in step: 4 x 65536 tokens of 8 heads
+// take 94 us in fp8 so, with 416 CTAs, and 106 with all 444.  Not below 5/6 of
+// the CTAs that fit; 256-byte rows do not need it, and int4, bound by its arithmetic, needs the CTAs.
+int grid_in_step(long long rows, int grid, int format, bool equal) {
+  if (!equal || (format != RA_CACHE_INT8 && format != RA_CACHE_FP8) || rows > grid) return grid;
+  const int whole = (int)(grid / rows * rows);
+  return 6 * whole >= 5 * grid ? whole : grid;
+}
+
+SegmentPlan plan_segment(bool prefix, int format, bool equal, int batch, int hq, int hkv, int tokens, int sms) {
   SegmentPlan s;
   memset(&s, 0, sizeof s);
   if (tokens <= 0) return s;
@@ -165,7 +175,8 @@ SegmentPlan plan_segment(bool prefix, int format, int batch, int hq, int hkv, in
   } else {
     const long long units = rows * ((tokens + kAttendTile - 1) / kAttendTile + kAttendRowUnits);
     s.grid = (int)std::min<long long>(units, (long long)attend_ctas(s.nq) * sms);
-    slots = (size_t)rows + s.grid;
+    slots = (size_t)rows + s.grid;      // room for the full grid, whatever the lengths
+    s.grid = grid_in_step(rows, s.grid, format, equal);
   }
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   s.ml_at = up(slots * s.qt * kHeadDim * sizeof(float));
@@ -209,8 +220,8 @@ size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, in
   const int sms = host_sm_count();
   size_t need = 0;
   for (int format : {RA_CACHE_FP16, RA_CACHE_INT4})
-    need = std::max(need, plan_segment(true, format, batch, num_q_heads, num_kv_heads, prefix_tokens, sms).bytes +
-                              plan_segment(false, format, batch, num_q_heads, num_kv_heads, cache_tokens, sms).bytes);
+    need = std::max(need, plan_segment(true, format, true, batch, num_q_heads, num_kv_heads, prefix_tokens, sms).bytes +
+                              plan_segment(false, format, true, batch, num_q_heads, num_kv_heads, cache_tokens, sms).bytes);
   return 256 + need;
 }
 
@@ -256,7 +267,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
     if (!has[i]) continue;
     const int format = (i ? p->cache : p->prefix).format;
     const SegmentPlan s =
-        plan_segment(i == 0, format, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
+        plan_segment(i == 0, format, i == 0 || !p->seq_lens, p->batch, p->num_q_heads, p->num_kv_heads, view[i].n_tokens, sms);
     float* part_o = reinterpret_cast<float*>(at);
     float* part_ml = reinterpret_cast<float*>(at + s.ml_at);
     CombineSegment& c = cp.seg[i];

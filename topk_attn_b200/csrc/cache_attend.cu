@@ -104,6 +104,13 @@ __device__ __forceinline__ void codes_of(uint32_t w, uint32_t& first, uint32_t& 
         : "r"(w));
   }
 }
+// The same pairs of an int8 word as fp16 subnormals of (code + 128) 2^-24: for the scores, whose sum of q
+// times 128 goes into the accumulators beforehand.  (For the values it would not do: their long sums
+// would lose in the difference.)
+__device__ __forceinline__ void int8_raw(uint32_t w, uint32_t& first, uint32_t& second) {
+  first = (w & 0x00ff00ffu) ^ 0x00800080u;
+  second = ((w >> 8) & 0x00ff00ffu) ^ 0x00800080u;
+}
 // Nibbles (i, i + 4) of a word hold code + 8.  raw: as they are, an fp16 subnormal of (code + 8) 2^-24,
 // the odd ones 16 times that; otherwise exact codes, the odd ones 16 times.
 __device__ __forceinline__ uint32_t nibbles_raw(uint32_t w, int i) {
@@ -332,7 +339,8 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     const long long slot = (long long)b * per_cache + row.inner + blockIdx.x;
     // B fragments of Q^T: column g is query q0 + 8 nq + g; the dims of lane t in the order K's lanes hold them
     uint32_t qb[NQ][8][2];
-    float k_off[NQ][FMT == kCacheInt4 ? 4 : 1][2];
+    constexpr int kOff = FMT == kCacheInt4 ? 4 : 1;
+    float k_off[NQ][kOff][2];
     float fac[NQ][2];      // what turns a raw score of my two columns into the log2 domain
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
@@ -388,21 +396,22 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
           constexpr float kOdd = FMT == kCacheInt4 ? 0.0625f : 1.f;     // K's odd nibbles come 16 times as large
           qb[nq][kk][1] = pack_pair<false>(y[i2] * down * kOdd, y[i2 + i1] * down * kOdd);
         }
-        if (FMT == kCacheInt4) {
-          // sum over a group of q (code + 8) less 8 times the sum of q: what the accumulators start from
+        if (FMT != kCacheFp8) {
+          // the sum of q (code + bias) less bias times the sum of q: what the accumulators start from
+          constexpr int kPer = 32 / kOff;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < kOff; ++j) {
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += x[8 * j + i];
+            for (int i = 0; i < kPer; ++i) sum += x[kPer * j + i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= down * (-8.f / 16777216.f);
+            sum *= down * (FMT == kCacheInt4 ? -8.f / 16777216.f : -128.f / 16777216.f);
             k_off[nq][j][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
             k_off[nq][j][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
           }
         }
-        const float up = __uint_as_float(top) * P.scale_log2e * (FMT == kCacheInt4 ? 16777216.f : 1.f);
+        const float up = __uint_as_float(top) * P.scale_log2e * (FMT == kCacheFp8 ? 1.f : 16777216.f);
         fac[nq][0] = __shfl_sync(0xffffffffu, up, 8 * t);
         fac[nq][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
       }
@@ -469,8 +478,8 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
             float part[NQ][4];
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
-              part[nq][0] = part[nq][2] = k_off[nq][FMT == kCacheInt4 ? j : 0][0];
-              part[nq][1] = part[nq][3] = k_off[nq][FMT == kCacheInt4 ? j : 0][1];
+              part[nq][0] = part[nq][2] = k_off[nq][j % kOff][0];
+              part[nq][1] = part[nq][3] = k_off[nq][j % kOff][1];
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -492,7 +501,13 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
           const int ta = r0 + g, tb = ta + 8;
           float y[NQ][4];
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) y[nq][0] = y[nq][1] = y[nq][2] = y[nq][3] = 0.f;
+          for (int nq = 0; nq < NQ; ++nq) {
+            y[nq][0] = y[nq][1] = y[nq][2] = y[nq][3] = 0.f;
+            if (FMT == kCacheInt8) {
+              x[nq][0] = x[nq][2] = k_off[nq][0][0];
+              x[nq][1] = x[nq][3] = k_off[nq][0][1];
+            }
+          }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint4 ua = lds128(kbase + ta * 128 + (((2 * t + half) ^ (ta & 7)) << 4));
@@ -501,8 +516,13 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t a[4];
-              codes_of<FMT>(wa[i], a[0], a[2]);
-              codes_of<FMT>(wb[i], a[1], a[3]);
+              if (FMT == kCacheInt8) {
+                int8_raw(wa[i], a[0], a[2]);
+                int8_raw(wb[i], a[1], a[3]);
+              } else {
+                codes_of<FMT>(wa[i], a[0], a[2]);
+                codes_of<FMT>(wb[i], a[1], a[3]);
+              }
               const int kk = 4 * half + i;
 #pragma unroll
               for (int nq = 0; nq < NQ; ++nq)
