@@ -216,8 +216,13 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   // loaded in the order of their first use: K of the first `stride` tiles, then V of tile j and K of
   // tile j + stride for each j, as far as there are any.
   const int stride = pair ? 1 : 2;
-  auto k_load = [&](int j) { return j + max(0, j - stride + 1); };
-  auto v_load = [&](int j) { return j + min(tiles, j + stride); };
+  // Each stream has stages of its own where it has tiles of its own: a barrier's parity tells two phases
+  // apart, so whoever waits for a stage's next load has to have waited for the one before it.
+  // Loads of a stream: K of its i-th tile is number 2 i, V number 2 i + 1.
+  const int per_stream = pair ? stages : stages / 2;
+  auto index_of = [&](int j, int v) { return 2 * (pair ? j : j >> 1) + v; };
+  auto stage_of = [&](int j, int v) { return index_of(j, v) % per_stream + (pair ? 0 : (j & 1) * per_stream); };
+  auto round_of = [&](int j, int v) { return (index_of(j, v) / per_stream) & 1; };
 
   if (tid == 0) {
     tma_prefetch_desc(&P.kmap);
@@ -261,31 +266,40 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfOtherRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA
-      const int ring = kCodes ? kCodeStages : stages;
       constexpr int kBytes = kCodes ? kCodeBytes : kPrefixTileBytes;
-      uint64_t* full = kCodes ? ctrl->code_full : ctrl->full;
-      uint64_t* empty = kCodes ? ctrl->code_empty : ctrl->empty;
-      int n = 0;
-      auto load = [&](const CUtensorMap* map, int tile) {
-        const int s = n % ring;
-        if (!wait(&empty[s], ((n / ring) & 1) ^ 1)) return false;
-        unsigned char* dst = (kCodes ? sm_codes : sm_kv) + s * kBytes;
+      int n = 0;                                     // loads so far
+      auto load = [&](int tile, int v) {
+        const int st = kCodes ? n % kCodeStages : stage_of(tile, v);
+        const unsigned round = kCodes ? (n / kCodeStages) & 1 : round_of(tile, v);
+        uint64_t* full = kCodes ? &ctrl->code_full[st] : &ctrl->full[st];
+        if (!wait(kCodes ? &ctrl->code_empty[st] : &ctrl->empty[st], round ^ 1)) return false;
+        unsigned char* dst = (kCodes ? sm_codes : sm_kv) + st * kBytes;
+        const CUtensorMap* map = v ? &P.vmap : &P.kmap;
         const int tok = (tile0 + tile) * kPrefixTile;
-        mbar_expect_tx(&full[s], kBytes);
-        tma_load_4d(dst, map, &full[s], 0, h, tok, 0);
-        if (!kCodes) tma_load_4d(dst + kPrefixHalf, map, &full[s], 64, h, tok, 0);
+        mbar_expect_tx(full, kBytes);
+        tma_load_4d(dst, map, full, 0, h, tok, 0);
+        if (!kCodes) tma_load_4d(dst + kPrefixHalf, map, full, 64, h, tok, 0);
         ++n;
         return true;
       };
       bool ok = true;
       for (int j = -stride; ok && j < tiles; ++j) {
-        if (j >= 0) ok = load(&P.vmap, j);
-        if (ok && j + stride < tiles) ok = load(&P.kmap, j + stride);
+        if (j >= 0) ok = load(j, 1);
+        if (ok && j + stride < tiles) ok = load(j + stride, 0);
       }
       // after a wait that ran out: no load may still be under way when the CTA ends
       if (!ok) {
-        int own = 0;
-        for (int i = max(0, n - ring); i < n; ++i) mbar_wait(&full[i % ring], (i / ring) & 1, &own);
+        int own = 0, i = 0;
+        auto settle = [&](int tile, int v) {
+          if (i < n && i + 6 >= n)                   // of the loads that may be under way
+            mbar_wait(kCodes ? &ctrl->code_full[i % kCodeStages] : &ctrl->full[stage_of(tile, v)],
+                      kCodes ? (i / kCodeStages) & 1 : round_of(tile, v), &own, kWaitLimitNs / 8);
+          ++i;
+        };
+        for (int j = -stride; i < n && j < tiles; ++j) {
+          if (j >= 0) settle(j, 1);
+          if (j + stride < tiles) settle(j + stride, 0);
+        }
       }
     } else if (warp == 1 || warp == 2) {
       // ---------------------------------------------------------------- MMA, stream warp - 1
@@ -298,9 +312,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       const uint64_t q_desc = tc_desc(smem_u32(sm_q) + (pair ? st * kPrefixTileBytes : 0), 16, 1024);
       const uint64_t k_desc = tc_desc(smem_u32(sm_kv), 16, 1024);
       const uint64_t v_desc = tc_desc(smem_u32(sm_kv), kPrefixHalf, 1024);
-      auto ready = [&](int n) { return wait(&ctrl->full[n % stages], (n / stages) & 1); };
+      auto ready = [&](int j, int v) { return wait(&ctrl->full[stage_of(j, v)], round_of(j, v)); };
       auto scores = [&](int j) {
-        const int s = k_load(j) % stages;
+        const int s = stage_of(j, 0);
         const uint64_t b = k_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         tc_fence_after();
         if (elect_one()) {
@@ -315,13 +329,13 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         __syncwarp();
       };
       int j = pair ? 0 : st;
-      bool ok = wait(&ctrl->q_full, 0) && (j >= tiles || ready(k_load(j)));
+      bool ok = wait(&ctrl->q_full, 0) && (j >= tiles || ready(j, 0));
       if (ok && j < tiles) scores(j);
       for (unsigned k = 0; ok && j < tiles; j += stride, ++k) {
         // the tiles first, so that the products follow one another once P is there
         const bool more = j + stride < tiles;
-        ok = ready(v_load(j)) && (!more || ready(k_load(j + stride)));
-        const int s = v_load(j) % stages;
+        ok = ready(j, 1) && (!more || ready(j + stride, 0));
+        const int s = stage_of(j, 1);
         const uint64_t b = v_desc + (uint64_t)(s * (kPrefixTileBytes >> 4));
         ok = ok && wait(&ctrl->p_full[st][0], k & 1);
         if (!ok) break;
@@ -362,23 +376,26 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     const int left = P.n_tokens - tile0 * kPrefixTile - t;       // tokens from mine on
     float ks = left > 0 ? __ldg(P.k_scale + at) : 0.f, vs = left > 0 ? __ldg(P.v_scale + at) : 0.f;
     // V of tile j and K of tile j + stride together: one round of waits, one fence
+    int n = 0;                                       // code tiles so far
     for (int j = -stride; j < tiles; ++j) {
       const int jk = j + stride, sj = jk % kScaleTiles;
       const bool has[2] = {j >= 0, jk < tiles};
-      const int load[2] = {v_load(j), k_load(jk)};
+      const int tile[2] = {max(j, 0), jk};
       bool go = true;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (has[i])
-          go = go && wait(&ctrl->code_full[load[i] % kCodeStages], (load[i] / kCodeStages) & 1) &&
-               wait(&ctrl->empty[load[i] % stages], ((load[i] / stages) & 1) ^ 1);
+      for (int i = 0, next = n; i < 2; ++i)
+        if (has[i]) {
+          go = go && wait(&ctrl->code_full[next % kCodeStages], (next / kCodeStages) & 1) &&
+               wait(&ctrl->empty[stage_of(tile[i], 1 - i)], round_of(tile[i], 1 - i) ^ 1);
+          ++next;
+        }
       if (!__all_sync(0xffffffffu, go)) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (!has[i]) continue;
-        const int c = load[i] % kCodeStages;
+        const int c = n++ % kCodeStages;
         const uint32_t src = smem_u32(sm_codes) + c * kCodeBytes + t * 128;
-        unsigned char* dst = sm_kv + (load[i] % stages) * kPrefixTileBytes;
+        unsigned char* dst = sm_kv + stage_of(tile[i], 1 - i) * kPrefixTileBytes;
         uint4 u[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) u[d] = lds128(src + ((d ^ (t & 7)) << 4));
@@ -394,11 +411,11 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       fence_proxy_async();
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (has[i]) mbar_arrive(&ctrl->full[load[i] % stages]);
+        if (has[i]) mbar_arrive(&ctrl->full[stage_of(tile[i], 1 - i)]);
       if (has[1]) {
         // both scales of tile jk.  Their slot of four was tile jk - 4's, whose weights are done: the stage
-        // of V of jk - stride, or of this K, was released by the product of a tile of jk - 4 or later of
-        // the same stream (of both, where both walk all tiles), and products follow their weights.
+        // of V of tile jk - stride had V of a tile of jk - 4 or later of the same stream, or K of one after
+        // it (of both streams, where both walk all tiles), and was released by a product behind them.
         scales->k[sj][t] = ks * P.scale_log2e;
         scales->v[sj][t] = vs;
         float top = fabsf(vs);
