@@ -193,6 +193,9 @@ template <int FMT, bool BF16>
 __global__ void __launch_bounds__(pf_threads(FMT >= kCacheInt8), 1)
 prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   constexpr bool kCodes = FMT >= kCacheInt8;
+  // fp16 results of 8-bit caches: the weights go through the product as an fp16 value and, in the other half
+  // of S's columns, the fp16 rest of it, so that the result's own rounding is the only one that counts
+  constexpr bool kRest = kCodes && !BF16;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -343,8 +346,10 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         const uint32_t add = k > 0;
         if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < kPrefixEarly / 16; ++c)
+          for (int c = 0; c < kPrefixEarly / 16; ++c) {
             tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, c > 0 ? 1u : add);
+            if (kRest) tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+          }
         }
         __syncwarp();
         ok = wait(&ctrl->p_full[st][1], k & 1);
@@ -352,8 +357,10 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int c = kPrefixEarly / 16; c < 8; ++c)
+          for (int c = kPrefixEarly / 16; c < 8; ++c) {
             tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+            if (kRest) tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+          }
           tc_commit(&ctrl->empty[s]);
           if (!more) tc_commit(&ctrl->o_full[st]);
         }
@@ -538,7 +545,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int part = 0; part < 4; ++part) {
-        uint32_t p[16];
+        uint32_t p[16], rest[kRest ? 16 : 1];
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
           const int e = 32 * part + 2 * c;
@@ -553,9 +560,14 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
             sum[d] = add2(sum[d], x);
             if (kCodes) x = mul2(x, d ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
             p[c + d] = pf_pack<BF16>(x.x, x.y);
+            if (kRest) {
+              const float2 y = h2f2(p[c + d]);
+              rest[kRest ? c + d : 0] = pf_pack<false>(x.x - y.x, x.y - y.y);
+            }
           }
         }
         tc_st16(tms + 16 * part, p);
+        if (kRest) tc_st16(tms + 64 + 16 * part, rest);
         if (part == kPrefixYield) mbar_arrive(&ctrl->turn[st ^ 1]);
         if (part == kPrefixEarly / 32 - 1 || part == 3) {
           tc_wait_st();
