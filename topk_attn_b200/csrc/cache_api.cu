@@ -171,7 +171,7 @@ SegmentPlan plan_segment(bool prefix, int format, bool equal, int batch, int hq,
   if (wide) {
     const int blocks = (s.query_tiles + 1) / 2 * hkv;
     s.splits = prefix_splits(blocks, (tokens + kPrefixTile - 1) / kPrefixTile, sms);
-    slots = (size_t)rows * 2 * s.splits;
+    slots = (size_t)rows * s.splits;
   } else {
     const long long units = rows * ((tokens + kAttendTile - 1) / kAttendTile + kAttendRowUnits);
     s.grid = (int)std::min<long long>(units, (long long)attend_ctas(s.nq) * sms);

@@ -800,40 +800,56 @@ cache_combine_kernel(const __grid_constant__ CombineParams P) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (r >= (long long)P.batch * P.hq) return;
   const int b = (int)(r / P.hq), hq = (int)(r % P.hq), h = hq / P.group;
-  float m = kNoMax, w = 0.f;
+  // the partials of either segment that are mine: [at, at + n) of the slots, strided by a row's query tile
+  long long at[2];
+  int n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const CombineSegment& G = P.seg[i];
+    at[i] = 0;
+    n[i] = 0;
+    if (!G.part_o) continue;
+    const int cache = G.prefix ? 0 : b;
+    if (G.lens && G.lens[cache] <= 0) continue;
+    const int qi = hq % P.group + (G.prefix ? b * P.group : 0);
+    const long long row = (long long)cache * P.hkv * G.query_tiles + h * G.query_tiles + qi / G.qt;
+    const int2 span = G.splits ? make_int2(0, G.splits - 1) : *reinterpret_cast<const int2*>(G.span + 2 * row);
+    const int parts = span.y - span.x + 1, per = (parts + WARPS - 1) / WARPS, mine = per * (warp % WARPS);
+    at[i] = ((G.splits ? row * G.splits : row) + span.x + mine) * G.qt + qi % G.qt;
+    n[i] = max(0, min(per, parts - mine));
+  }
+  // maxima and weights of the first 32 of both under way together
+  float2 ml[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    ml[i] = make_float2(kNoMax, 0.f);
+    if (lane < n[i]) ml[i] = *reinterpret_cast<const float2*>(P.seg[i].part_ml + 2 * (at[i] + (long long)lane * P.seg[i].qt));
+  }
+  float m = fmaxf(ml[0].x, ml[1].x), w = 0.f;
+#pragma unroll
+  for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const CombineSegment& G = P.seg[i];
-    if (!G.part_o) continue;
-    const int cache = G.prefix ? 0 : b;
-    const int qi = hq % P.group + (G.prefix ? b * P.group : 0);
-    const long long row = (long long)cache * P.hkv * G.query_tiles + h * G.query_tiles + qi / G.qt;
-    if (G.lens && G.lens[cache] <= 0) continue;
-    int2 span;
-    long long slot0 = row;
-    if (G.splits) {
-      slot0 = row * 2 * G.splits;
-      span = make_int2(0, (((qi / G.qt) | 1) < G.query_tiles ? G.splits : 2 * G.splits) - 1);
-    } else {
-      span = *reinterpret_cast<const int2*>(G.span + 2 * row);
-    }
-    const int c1 = span.y, per = min(32, (span.y - span.x + WARPS) / WARPS);
-    const long long e0 = slot0 * G.qt + qi % G.qt;
-    for (int c = span.x + per * (warp % WARPS); c <= c1; c += per * WARPS) {
-      const int n = min(per, c1 - c + 1);
-      float2 ml = make_float2(kNoMax, 0.f);
-      if (lane < n) ml = *reinterpret_cast<const float2*>(G.part_ml + 2 * (e0 + (long long)(c + lane) * G.qt));
-      float top = fmaxf(m, ml.x);
+    for (int c = 0; c < n[i]; c += 32) {
+      if (c) {           // a row of more than 32 partials to a warp: one long context alone
+        ml[i] = make_float2(kNoMax, 0.f);
+        if (c + lane < n[i]) ml[i] = *reinterpret_cast<const float2*>(G.part_ml + 2 * (at[i] + (long long)(c + lane) * G.qt));
+        float top = fmaxf(m, ml[i].x);
 #pragma unroll
-      for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-      const float keep = fast_exp2(m - top), f = fast_exp2(ml.x - top);
-      m = top;
-      w = w * keep + ml.y * f;           // of this lane's partials; summed over the lanes at the end
-      sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
-      const float* src = G.part_o + (e0 + (long long)c * G.qt) * kHeadDim + 4 * lane;
+        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float keep = fast_exp2(m - top);
+        m = top;
+        w *= keep;
+        sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+      }
+      const float f = fast_exp2(ml[i].x - m);
+      w += ml[i].y * f;              // of this lane's partials; summed over the lanes at the end
+      const float* src = G.part_o + (at[i] + (long long)c * G.qt) * kHeadDim + 4 * lane;
+      const int here = min(32, n[i] - c);
 #pragma unroll 8
-      for (int k = 0; k < n; ++k) {
+      for (int k = 0; k < here; ++k) {
         const float4 v = *reinterpret_cast<const float4*>(src + (long long)k * G.qt * kHeadDim);
         const float fk = __shfl_sync(0xffffffffu, f, k);
         sum.x += v.x * fk; sum.y += v.y * fk; sum.z += v.z * fk; sum.w += v.w * fk;

@@ -52,8 +52,7 @@ struct CombineSegment {
   const int* span;
   const int* lens;
   int query_tiles, qt, prefix;
-  int splits;               // > 0: a row's partials lie in 2 * splits slots of its own, of which a query
-                            // tile that has a partner uses the first half
+  int splits;               // > 0: a row's partials lie in so many slots of its own
 };
 struct CombineParams {
   CombineSegment seg[2];

@@ -6,7 +6,7 @@
 // A CTA takes one kv head, up to two tiles of 128 queries and a range of the tokens.  It runs two
 // streams, each with its own S and O in TMEM and its own softmax warpgroup, so that the tensor cores
 // work on one while the other's softmax runs.  With two query tiles both streams walk the same K/V
-// tiles; with one, they take the tiles in turn and leave a partial each.
+// tiles; with one, they take the tiles in turn and join their sums at the end.
 //   warp 0      TMA: K and V tiles of 32 KiB in one ring
 //   warps 1, 2  one thread of each issues a stream's MMAs; its commits release tiles and hand over S
 //   warps 12-15 for 8-bit caches: codes into fp16 or bf16 tiles, and the scales beside them; a token's K
@@ -579,44 +579,81 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     }
     // ---------------------------------------------------------------- partial
     const int qt = pair ? qt0 + st : qt0;
-    const long long slot = ((long long)h * P.query_tiles + qt) * (2 * P.splits) + (pair ? split : 2 * split + st);
+    const long long slot = ((long long)h * P.query_tiles + qt) * P.splits + split;
     const int row0 = (warp & 3) * 32;                      // my warp's rows
+    const int live = P.queries - qt * kPrefixTile - row0;  // of them, how many are queries
+    float* out = P.part_o + (slot * kPrefixTile + row0) * kHeadDim;
     if (k && ok) {
       wait(&ctrl->o_full[st], 0);
       __syncwarp();
       tc_fence_after();
     }
-    // 32 rows x 32 dims at a time through shared memory, so that rows leave in whole lines: in the stream's
-    // query tile, or in the one that both read once both are done
-    if (!pair) asm volatile("bar.sync 2, 256;" ::: "memory");
-    const uint32_t buf = smem_u32(sm_q) + (pair ? st * kPrefixTileBytes + (warp & 3) * 4096 : (warp - 4) * 4096);
-    const int live = P.queries - qt * kPrefixTile - row0;  // rows of mine that are queries
-    float* out = P.part_o + (slot * kPrefixTile + row0) * kHeadDim;
-#pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
-      uint32_t o[32];
-      if (k) {
-        tc_ld32(o, tmo + c);
-        tc_wait_ld();
-      } else {
-#pragma unroll
-        for (int d = 0; d < 32; ++d) o[d] = 0u;
-      }
+    auto stage = [&](uint32_t buf, const uint32_t* o) {    // 32 dims of my row; a row is 128 bytes, swizzled
 #pragma unroll
       for (int d = 0; d < 8; ++d)
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(buf + lane * 128 + ((d ^ (lane & 7)) << 4)),
                      "r"(o[4 * d]), "r"(o[4 * d + 1]), "r"(o[4 * d + 2]), "r"(o[4 * d + 3])
                      : "memory");
-      __syncwarp();
+    };
+    if (pair) {
+      // 32 rows x 32 dims at a time through the stream's query tile, so that rows leave in whole lines
+      const uint32_t buf = smem_u32(sm_q) + st * kPrefixTileBytes + (warp & 3) * 4096;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t o[32];
+        tc_ld32(o, tmo + c);
+        tc_wait_ld();
+        stage(buf, o);
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), d = lane & 7;
-        const uint4 v = lds128(buf + r * 128 + ((d ^ (r & 7)) << 4));
-        if (r < live) *reinterpret_cast<uint4*>(out + r * kHeadDim + c + 4 * d) = v;
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3), d = lane & 7;
+          const uint4 v = lds128(buf + r * 128 + ((d ^ (r & 7)) << 4));
+          if (r < live) *reinterpret_cast<uint4*>(out + r * kHeadDim + c + 4 * d) = v;
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      *reinterpret_cast<float2*>(P.part_ml + (slot * kPrefixTile + row0 + lane) * 2) = make_float2(m_ref, l);
+    } else {
+      // both streams saw the same queries: their sums are joined here, through the ring, where nothing is
+      // under way once both are done
+      float2* sm_ml = reinterpret_cast<float2*>(sm_q);     // [2][128]
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      sm_ml[st * kPrefixTile + row0 + lane] = make_float2(m_ref, l);
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      const float2 other = sm_ml[(st ^ 1) * kPrefixTile + row0 + lane];
+      const float top = fmaxf(m_ref, other.x), f = fast_exp2(m_ref - top);
+      const uint32_t buf = smem_u32(sm_kv) + (warp & 3) * 16384;   // [4 blocks of 32 dims][32 rows]; stream 1 at + 64 KiB
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (k) {
+          tc_ld32(o, tmo + 32 * c);
+          tc_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
+        } else {
+#pragma unroll
+          for (int d = 0; d < 32; ++d) o[d] = 0u;
+        }
+        stage(buf + st * 65536 + c * 4096, o);
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      // half of the 32 rows each
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int c = i & 3, r = 16 * st + 4 * (i >> 2) + (lane >> 3), d = lane & 7;
+        const uint32_t at = buf + c * 4096 + r * 128 + ((d ^ (r & 7)) << 4);
+        const uint4 x = lds128(at), y = lds128(at + 65536);
+        if (r < live)
+          *reinterpret_cast<float4*>(out + r * kHeadDim + 32 * c + 4 * d) =
+              make_float4(__uint_as_float(x.x) + __uint_as_float(y.x), __uint_as_float(x.y) + __uint_as_float(y.y),
+                          __uint_as_float(x.z) + __uint_as_float(y.z), __uint_as_float(x.w) + __uint_as_float(y.w));
+      }
+      if (st == 0)
+        *reinterpret_cast<float2*>(P.part_ml + (slot * kPrefixTile + row0 + lane) * 2) =
+            make_float2(top, l * f + other.y * fast_exp2(other.x - top));
     }
-    *reinterpret_cast<float2*>(P.part_ml + (slot * kPrefixTile + row0 + lane) * 2) = make_float2(m_ref, l);
     tc_fence_before();
   }
   __syncthreads();

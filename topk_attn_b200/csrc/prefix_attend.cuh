@@ -14,7 +14,7 @@ struct PrefixAttendParams {
   const float* k_scale;     // of codes: [hkv][tokens], scale_hstride floats between heads
   const float* v_scale;
   long long scale_hstride;
-  float* part_o;            // [(kv head, query tile)][2 splits][128][128] un-normalised sums
+  float* part_o;            // [(kv head, query tile)][splits][128][128] un-normalised sums
   float* part_ml;           // same, [2]: maximum (log2 domain), weight
   unsigned* status;
   int n_tokens, queries;    // queries of a kv head: batch * group
