@@ -273,6 +273,53 @@ def test_captured_graphs_replayed_at_the_same_time_and_other_streams():
     ops.check_status(torch.device(DEV))
 
 
+def test_first_calls_of_a_process_inside_a_capture():
+    """A process whose very first calls are captured: scratch and status come from the graph's memory."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from topk_attn_b200 import ops
+torch.manual_seed(0)
+q = torch.randn(40, 8, 128, device="cuda", dtype=torch.float16)
+pk, pv = (torch.randn(300, 2, 128, device="cuda", dtype=torch.float16) for _ in range(2))
+cache = ops.quantized_kv_cache(64, 2, "int8", batch=40)
+rows = torch.randn(40, 9, 2, 128, device="cuda", dtype=torch.float16)
+lens = torch.full((40,), 9, device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ops.kv_append_quantized(cache, rows, rows, 0)
+    a = ops.flash_decoding_quantized(q, cache, 0.1, lens)
+    b = ops.shared_prefix_attention(q, (pk, pv), None, 0.1)
+for _ in range(3):
+    g.replay()
+torch.cuda.synchronize()
+assert torch.equal(a, ops.flash_decoding_quantized(q, cache, 0.1, lens))
+assert torch.equal(b, ops.shared_prefix_attention(q, (pk, pv), None, 0.1))
+ops.check_status()
+print("captured first")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "captured first" in res.stdout, res.stderr[-2000:]
+
+
+def test_output_in_place_of_the_queries_and_another_stream():
+    from topk_attn_b200 import ops
+    q, prefix, own = make(20, 8, 2, 700, 90, "", torch.float16, 11)
+    pre, cache = device_cache(prefix, ""), device_cache(own, "")
+    ref = ops.shared_prefix_attention(q.to(DEV), pre, cache, SM)
+    dq = q.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ops.shared_prefix_attention(dq, pre, cache, SM, out=dq)
+    torch.cuda.synchronize()
+    assert out.data_ptr() == dq.data_ptr() and torch.equal(dq, ref)
+
+
 def test_refusals():
     from topk_attn_b200 import capi, ops
     q, prefix, own = make(2, 8, 2, 50, 40, "", torch.float16, 1)

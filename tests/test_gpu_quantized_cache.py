@@ -139,6 +139,17 @@ def test_padded_batch_counts_and_rows_behind_are_left_alone(kind):
     check(cache, at.tolist(), v, 1, counts)
 
 
+def test_a_padded_batch_may_reach_over_the_end_of_the_cache():
+    """With an int position the rows that counts leaves out need no room."""
+    from topk_attn_b200 import ops
+    k = rows((2, 8, 3, 128), torch.float16, 1)
+    counts = torch.tensor([2, 0], dtype=torch.int32)
+    cache = ops.quantized_kv_cache(10, 3, "fp8", batch=2, device=DEV)
+    ops.kv_append_quantized(cache, k.to(DEV), k.to(DEV), 8, counts.to(DEV))
+    ops.check_status(torch.device(DEV))
+    check(cache, [8, 8], k, 0, counts)
+
+
 def test_rows_outside_the_cache_are_left_out_and_reported():
     from topk_attn_b200 import capi, ops
     dev = torch.device(DEV)

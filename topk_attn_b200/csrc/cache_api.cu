@@ -20,6 +20,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 int invalid(const char* why) { return host_fail(RA_ERR_INVALID_ARGUMENT, why); }
 int unsupported(const char* why) { return host_fail(RA_ERR_UNSUPPORTED, why); }
 
+constexpr int kMaxTokens = INT32_MAX - 4095;   // tiles are counted in 32 bits, rounding up
+
 bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
 // Checks a cache description and turns it into the kernels' view of it.
@@ -27,6 +29,7 @@ int view_of(const ra_kv_cache& c, bool per_row, int caches, CacheView& v) {
   if (c.format < RA_CACHE_FP16 || c.format > RA_CACHE_INT4) return invalid("unknown cache format");
   if (!c.k || !c.v) return invalid("a cache pointer is null");
   if (misaligned(c.k, 16) || misaligned(c.v, 16)) return invalid("cache pointers must be 16-byte aligned");
+  if (c.num_tokens > kMaxTokens) return unsupported("more than 2^31 - 4096 tokens in a cache");
   const long long esz = c.format <= RA_CACHE_BF16 ? 2 : 1;
   const int row = cache_row_bytes(c.format);
   v.k = static_cast<unsigned char*>(c.k);
@@ -193,7 +196,8 @@ int ra_kv_append_quantized(const ra_kv_rows_params* p) {
   QuantParams q;
   const int st = check_rows(p, q);
   if (st != RA_OK) return st;
-  if (!p->positions && (p->position < 0 || (int64_t)p->position + p->num_rows > p->cache.num_tokens))
+  // counts may keep the last rows of a padded batch out of the cache's end: then the kernel looks
+  if (!p->positions && (p->position < 0 || (!p->counts && (int64_t)p->position + p->num_rows > p->cache.num_tokens)))
     return invalid("rows outside the cache");
   if (p->num_rows == 0) return RA_OK;
   const cudaError_t e = launch_kv_quantize(q, p->cache.format, p->row_type == RA_TYPE_BF16,
