@@ -266,6 +266,10 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   cp.hq = p->num_q_heads;
   cp.hkv = p->num_kv_heads;
   cp.group = p->num_q_heads / p->num_kv_heads;
+  // The first kernel's launch overlaps the end of whatever runs before it, except in a capture, where what
+  // is before it need not be a kernel.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  const bool early = cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone;
   char* at = static_cast<char*>(p->workspace);
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;
@@ -309,6 +313,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
       a.hkv = p->num_kv_heads;
       a.group = cp.group;
       a.splits = s.splits;
+      a.early = early;
       a.scale_log2e = p->sm_scale * kLog2e;
       const cudaError_t e = launch_prefix_attend(a, format, bf16, stream);
       if (e != cudaSuccess) return host_cuda_fail(e, "prefix_attend launch");
@@ -335,6 +340,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
     a.hkv = p->num_kv_heads;
     a.group = cp.group;
     a.after = i == 1 && has[0];
+    a.early = a.after || early;
     a.scale_log2e = p->sm_scale * kLog2e;
     const cudaError_t e = launch_cache_attend(a, format, bf16, s.nq, stream);
     if (e != cudaSuccess) return host_cuda_fail(e, "cache_attend launch");

@@ -166,6 +166,8 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
     ctrl->timeout = 0;
     fence_barrier_init();
   }
+  // a call's first kernel is launched while the one before it still runs, and touches no memory before this
+  if (!P.after) asm volatile("griddepcontrol.wait;" ::: "memory");
   auto length_of = [&](int b) {
     int len = G.cache.n_tokens;
     if (G.lens) len = max(0, min(len, G.lens[b]));
@@ -797,6 +799,7 @@ cache_combine_kernel(const __grid_constant__ CombineParams P) {
   __shared__ float2 sm_ml[kCombineWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long r = (long long)blockIdx.x * (kCombineWarps / WARPS) + warp / WARPS;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the next call's first kernel, which waits too
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (r >= (long long)P.batch * P.hq) return;
   const int b = (int)(r / P.hq), hq = (int)(r % P.hq), h = hq / P.group;
@@ -909,7 +912,7 @@ cudaError_t launch_one(const CacheAttendParams& P, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = P.after ? 1 : 0;
+  cfg.numAttrs = P.early ? 1 : 0;
   note_launch();
   return cudaLaunchKernelEx(&cfg, kern, P);
 }

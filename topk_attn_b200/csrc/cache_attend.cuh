@@ -43,6 +43,7 @@ struct CacheAttendParams {
   float scale_log2e;
   int after;                // launched while the prefix's kernel still runs: needs nothing of it, but
                             // ends behind it, so that the combine need only wait for this one
+  int early;                // launched with the programmatic attribute
 };
 
 // What the combine reads of a segment.

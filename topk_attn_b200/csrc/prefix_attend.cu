@@ -255,6 +255,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // nothing of the kernels before is touched before this; and what is launched after this one, which may
+  // not wait for it, must not start before it has passed
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = ctrl->tmem;
   // TMEM columns of stream st: S at 128 st, P in its first half; O at 256 + 128 st
@@ -673,9 +676,18 @@ cudaError_t launch_one(const PrefixAttendParams& P, cudaStream_t stream) {
   const cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return e;
   const int blocks = (P.query_tiles + 1) / 2 * P.hkv * P.splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(pf_threads(kCodes));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = P.early ? 1 : 0;
   note_launch();
-  kern<<<blocks, pf_threads(kCodes), smem, stream>>>(P);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kern, P);
 }
 
 }  // namespace

@@ -22,6 +22,7 @@ struct PrefixAttendParams {
   int hq, hkv, group;
   int splits;
   float scale_log2e;
+  int early;                // launched while the kernel before it still runs
 };
 
 // format: not int4, whose scales lie along the dims and cannot be applied to S
