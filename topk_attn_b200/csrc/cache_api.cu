@@ -60,6 +60,13 @@ int view_of(const ra_kv_cache& c, bool per_row, int caches, CacheView& v) {
   return RA_OK;
 }
 
+// A call's first kernel is launched so that its launch overlaps the end of whatever runs before it (it waits
+// for that end itself), except in a capture, where what is before it need not be a kernel.
+bool capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone;
+}
+
 int check_rows(const ra_kv_rows_params* p, QuantParams& q) {
   if (!p) return invalid("params is null");
   if (p->head_dim != kHeadDim) return unsupported("head_dim must be 128");
@@ -200,6 +207,7 @@ int ra_kv_append_quantized(const ra_kv_rows_params* p) {
   if (!p->positions && (p->position < 0 || (!p->counts && (int64_t)p->position + p->num_rows > p->cache.num_tokens)))
     return invalid("rows outside the cache");
   if (p->num_rows == 0) return RA_OK;
+  q.early = !capturing(static_cast<cudaStream_t>(p->stream));
   const cudaError_t e = launch_kv_quantize(q, p->cache.format, p->row_type == RA_TYPE_BF16,
                                            static_cast<cudaStream_t>(p->stream));
   return e == cudaSuccess ? RA_OK : host_cuda_fail(e, "kv_append_quantized launch");
@@ -212,6 +220,7 @@ int ra_kv_dequantize(const ra_kv_rows_params* p) {
   if (!p->positions && (p->position < 0 || (int64_t)p->position + p->num_rows > p->cache.num_tokens))
     return invalid("rows outside the cache");
   if (p->num_rows == 0) return RA_OK;
+  q.early = !capturing(static_cast<cudaStream_t>(p->stream));
   const cudaError_t e = launch_kv_dequantize(q, p->cache.format, p->row_type == RA_TYPE_BF16,
                                              static_cast<cudaStream_t>(p->stream));
   return e == cudaSuccess ? RA_OK : host_cuda_fail(e, "kv_dequantize launch");
@@ -266,10 +275,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   cp.hq = p->num_q_heads;
   cp.hkv = p->num_kv_heads;
   cp.group = p->num_q_heads / p->num_kv_heads;
-  // The first kernel's launch overlaps the end of whatever runs before it, except in a capture, where what
-  // is before it need not be a kernel.
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  const bool early = cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone;
+  const bool early = !capturing(stream);
   char* at = static_cast<char*>(p->workspace);
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;

@@ -9,6 +9,7 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -188,6 +189,22 @@ int kv_rows(bool back, const Tensor& ck, const Tensor& cv, const Tensor& cks, co
   return back ? ra_kv_dequantize(&p) : ra_kv_append_quantized(&p);
 }
 
+// count tokens of every cache as new tensors: (status, k, v)
+std::tuple<int, Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
+                                        const OptTensor& positions, int64_t position, int64_t count, bool bf16) {
+  if (!ck.is_cuda()) refuse("tensors must be CUDA tensors");
+  if (ck.dim() != 3 && ck.dim() != 4) refuse("k and v must be [B,N,Hkv,128] or [N,Hkv,128]");
+  if (count < 0) refuse("count must not be negative");
+  std::vector<int64_t> shape(ck.sizes().begin(), ck.sizes().end());
+  shape[shape.size() - 3] = count;
+  shape.back() = 128;
+  const auto opt = torch::TensorOptions().dtype(bf16 ? at::kBFloat16 : at::kHalf).device(ck.device());
+  const c10::cuda::CUDAGuard guard(ck.device());
+  Tensor k = torch::empty(shape, opt), v = torch::empty(shape, opt);
+  const int st = count ? kv_rows(true, ck, cv, cks, cvs, k, v, positions, position, OptTensor()) : RA_OK;
+  return {st, k, v};
+}
+
 std::pair<int, Tensor> cache_attention(const Tensor& q, const OptTensor& pk, const OptTensor& pv, const OptTensor& pks,
                                        const OptTensor& pvs, const OptTensor& k, const OptTensor& v,
                                        const OptTensor& ks, const OptTensor& vs, const OptTensor& seq_lens,
@@ -253,6 +270,7 @@ OptTensor status_block(int64_t device) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_rows", &kv_rows, "Rows into a quantised cache, or back out of it; the C ABI's status");
+  m.def("kv_read", &kv_read, "Tokens of a quantised cache as new tensors: (status, k, v)");
   m.def("cache_attention", &cache_attention, "Attention over a shared prefix and own caches: (status, out)");
   m.def("status_block", &status_block, "A device's status block, or None before the first call there");
 }

@@ -84,6 +84,8 @@ struct RowWalk {
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(kQuantThreads)
 kv_quantize_kernel(const __grid_constant__ QuantParams P) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ float sm_scale[];               // [heads][tokens][scales of a row]
   constexpr int kScales = cache_row_scales(FMT);
   constexpr int kDeep = 2;                          // rows whose loads are under way together
@@ -242,6 +244,9 @@ __device__ __forceinline__ void values_of(uint2 u, float s, float (&x)[8]) {
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(kQuantThreads)
 kv_dequantize_kernel(const __grid_constant__ QuantParams P) {
+  // launched while the kernel before it still runs
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ float sm_scale[];               // [heads][tokens][scales of a row]
   constexpr int kScales = cache_row_scales(FMT);
   constexpr int kDeep = 4;
@@ -324,15 +329,22 @@ cudaError_t launch_one(QuantParams P, bool bf16, bool back, cudaStream_t stream)
   P.tile = quant_tile(P);
   const size_t smem = (size_t)P.tile * P.heads * cache_row_scales(FMT) * sizeof(float);
   const dim3 grid((unsigned)((P.n_rows + P.tile - 1) / P.tile), 2, (unsigned)P.caches);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kQuantThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = P.early ? 1 : 0;
   note_launch();
-  if (back) {
-    if (bf16) kv_dequantize_kernel<FMT, true><<<grid, kQuantThreads, smem, stream>>>(P);
-    else kv_dequantize_kernel<FMT, false><<<grid, kQuantThreads, smem, stream>>>(P);
-  } else {
-    if (bf16) kv_quantize_kernel<FMT, true><<<grid, kQuantThreads, smem, stream>>>(P);
-    else kv_quantize_kernel<FMT, false><<<grid, kQuantThreads, smem, stream>>>(P);
-  }
-  return cudaGetLastError();
+  if (back)
+    return bf16 ? cudaLaunchKernelEx(&cfg, kv_dequantize_kernel<FMT, true>, P)
+                : cudaLaunchKernelEx(&cfg, kv_dequantize_kernel<FMT, false>, P);
+  return bf16 ? cudaLaunchKernelEx(&cfg, kv_quantize_kernel<FMT, true>, P)
+              : cudaLaunchKernelEx(&cfg, kv_quantize_kernel<FMT, false>, P);
 }
 
 cudaError_t launch_format(const QuantParams& P, int format, bool bf16, bool back, cudaStream_t stream) {

@@ -40,6 +40,7 @@ struct QuantParams {
   const int* positions;     // [caches] or null
   int position;
   const int* counts;        // [caches] or null
+  int early;                // launched while the kernel before it still runs, which the kernel waits for
   unsigned* status;
 };
 

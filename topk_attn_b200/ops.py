@@ -360,18 +360,13 @@ def kv_dequantize(cache: QuantizedKV, position: Union[int, Tensor] = 0, count: O
     device-side position puts outside the cache read as zeros and are reported by ``check_status``."""
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("dtype must be float16 or bfloat16")
-    if not cache.k.is_cuda:
-        raise ValueError("tensors must be CUDA tensors")
     at, pos = (position, 0) if isinstance(position, Tensor) else (None, int(position))
     if count is None:
         if at is not None:
             raise ValueError("a position on the device needs a count")
         count = cache.num_tokens - pos
-    if count < 0:
-        raise ValueError("count must not be negative")
-    shape = (*cache.k.shape[:-3], count, cache.k.size(-2), 128)
-    k, v = torch.empty(shape, dtype=dtype, device=cache.k.device), torch.empty(shape, dtype=dtype, device=cache.k.device)
-    st = _cache_ops().kv_rows(True, cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, at, pos, None)
+    st, k, v = _cache_ops().kv_read(cache.k, cache.v, cache.k_scale, cache.v_scale, at, pos, count,
+                                    dtype == torch.bfloat16)
     if st:
         capi.check(st)
     return k, v
