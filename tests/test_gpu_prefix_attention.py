@@ -204,6 +204,38 @@ def test_repeated_calls_give_the_same_bits_and_strided_caches_work():
     assert torch.equal(ops.shared_prefix_attention(q.to(DEV), device_cache(prefix, ""), hm, SM), first)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,Hkv,Np,N", [(32, 8, 16385, 200), (150, 2, 9000, 70), (3, 4, 6000, 900)])
+def test_calls_behind_one_another_give_the_same_bits(kind, B, Hkv, Np, N):
+    """Many calls without a pause, on two sets of inputs in turn, all of them in L2: a tile that is overwritten
+    too early, or a call that overlaps the next one's memory, shows as another result."""
+    from topk_attn_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(7)
+    sets = []
+    for _ in range(2):
+        q = torch.randn(B, 4 * Hkv, 128, generator=g, device=DEV).half()
+        rows = [torch.randn(Np, Hkv, 128, generator=g, device=DEV).half() for _ in range(2)]
+        own = [torch.randn(B, N, Hkv, 128, generator=g, device=DEV).half() for _ in range(2)]
+        if kind:
+            pre = ops.quantized_kv_cache(Np, Hkv, kind, device=DEV)
+            ops.kv_append_quantized(pre, *rows, 0)
+            cache = ops.quantized_kv_cache(N, Hkv, kind, batch=B, device=DEV)
+            ops.kv_append_quantized(cache, *own, 0)
+        else:
+            pre, cache = tuple(rows), tuple(own)
+        lens = torch.randint(0, N + 1, (B,), generator=g, device=DEV, dtype=torch.int32)
+        torch.cuda.synchronize()
+        sets.append((q, pre, cache, SM, lens))
+    want = []
+    for s in sets:
+        want.append(ops.shared_prefix_attention(*s))
+        torch.cuda.synchronize()
+    for _ in range(6):
+        got = [ops.shared_prefix_attention(*sets[i % 2]) for i in range(60)]
+        assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
+    ops.check_status(torch.device(DEV))
+
+
 def test_a_decode_loop_over_a_quantised_prefix_and_cache():
     """The operators together: a prompt is quantised once into a shared cache, then every step appends one
     token to each row's own cache and attends over both; and reading the caches back gives what the

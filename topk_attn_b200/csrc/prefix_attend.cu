@@ -409,7 +409,6 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         uint4 u[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) u[d] = lds128(src + ((d ^ (t & 7)) << 4));
-        mbar_arrive(&ctrl->code_empty[c]);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           uint32_t r[8];
@@ -417,6 +416,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
           *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d)) = make_uint4(r[0], r[1], r[2], r[3]);
           *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
         }
+        // only now: a barrier's arrival does not wait for shared loads that nothing has used yet, and the
+        // next tile of codes, when it comes from L2, overtook them
+        mbar_arrive(&ctrl->code_empty[c]);
       }
       fence_proxy_async();
 #pragma unroll
