@@ -155,12 +155,13 @@ int prefix_splits(int blocks, int tiles, int sms) {
   return best;
 }
 
-// Where every cache is equally long and is held in 8 bits, the grid is a multiple of the rows, so that the
-// heads, whose 128-byte rows lie side by side in memory, are walked in step: 4 x 65536 tokens of 8 heads
-// take 94 us in fp8 so, with 416 CTAs, and 106 with all 444.  Not below 5/6 of
-// the CTAs that fit; 256-byte rows do not need it, and int4, bound by its arithmetic, needs the CTAs.
+// Where every cache is equally long and held in fp8, the grid is a multiple of the rows, so that the heads,
+// whose 128-byte rows lie side by side in memory, are walked in step: 8 x 32768 tokens of 8 heads take 95 us
+// so, with 384 CTAs, and 104 with all 444 (with 4 heads 93 and 90).  Not below 5/6 of the CTAs that fit.
+// 256-byte rows do not need it; int8 and int4, bound by their arithmetic, need the CTAs (int8: 113 against
+// 102).
 int grid_in_step(long long rows, int grid, int format, bool equal) {
-  if (!equal || (format != RA_CACHE_INT8 && format != RA_CACHE_FP8) || rows > grid) return grid;
+  if (!equal || format != RA_CACHE_FP8 || rows > grid) return grid;
   const int whole = (int)(grid / rows * rows);
   return 6 * whole >= 5 * grid ? whole : grid;
 }

@@ -141,8 +141,8 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
   constexpr int kScaleFloats = attend_scale_floats(FMT);
   // fp16 results of 8-bit caches: the weights go through the product as an fp16 value and the fp16 rest of
   // it.  Rounded once they would add as much error again as the result's own rounding (2.0e-4 of its norm
-  // each, 3.1e-4 together over 32768 tokens).  The eight more MMAs cost 9 % of the time: 8 x 32768 tokens of
-  // int8 take 113 us with them and 104 without.
+  // each, 3.1e-4 together over 32768 tokens).  The eight more MMAs cost up to 9 % of the time (int8, 8 x
+  // 32768 tokens on 384 CTAs: 113 us with them, 104 without).
   constexpr bool kRest = !kDense && !BF16 && kNS == 1;
   constexpr int QT = 8 * NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
