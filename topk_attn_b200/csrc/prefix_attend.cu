@@ -15,6 +15,13 @@
 //               P goes back into S's columns as the A operand of the second product
 // The maximum moves only when a score exceeds it by 2^4, and only then O is rescaled in TMEM; no wait
 // is needed for that: S(k) is committed after O's product k-1.  Weights are rounded to the type of V.
+//
+// 256 batch rows x 32 heads behind 32768 bf16 tokens of 8 kv heads: 134-150 us for this kernel, 0.92-1.03
+// PFLOP/s, with the tensor pipe at 49 %: a pair of steps takes about 3050 cycles, 2048 of them products, and
+// what bounds it is each stream's chain of S, maximum, exponentials (about 1300 cycles for 128 x 128 on the
+// 16 results a clock of the special-function unit) and O.  Computing a share of the exponentials on the FMA
+// pipe changed nothing, handing P over in four parts instead of two made it slower (170 against 149 us).
+// With 128 queries and 16385 int8 tokens it takes about 30 us, bound by the conversion of codes.
 #include "prefix_attend.cuh"
 
 #include "api_host.cuh"
@@ -34,7 +41,9 @@ __host__ __device__ constexpr int pf_threads(bool codes) { return codes ? 512 : 
 __host__ __device__ constexpr int pf_soft_regs(bool codes) { return codes ? 184 : 232; }
 constexpr int kPfOtherRegs = 40, kPfConvertRegs = 104;
 constexpr int kPrefixEarly = 64;                // tokens of P whose product starts while the rest is computed
-constexpr int kPrefixYield = 2;                 // quarter of P after which the other stream's turn begins
+// Quarter of P after which the other stream's turn at the exponentials begins: 145 us at the sizes above
+// against 146 with the last quarter, 167 with the second.
+constexpr int kPrefixYield = 2;
 constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f;
 
 struct PrefixScales {
