@@ -202,9 +202,9 @@ template <int FMT, bool BF16>
 __global__ void __launch_bounds__(pf_threads(FMT >= kCacheInt8), 1)
 prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   constexpr bool kCodes = FMT >= kCacheInt8;
-  // fp16 results of 8-bit caches: the weights go through the product as an fp16 value and, in the other half
-  // of S's columns, the fp16 rest of it, so that the result's own rounding is the only one that counts
-  constexpr bool kRest = kCodes && !BF16;
+  // 8-bit caches: the weights go through the product as an fp16 (bf16) value and, in the other half of S's
+  // columns, the rest of it in the same type, so that the result's own rounding is the only one that counts
+  constexpr bool kRest = kCodes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -575,8 +575,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
             if (kCodes) x = mul2(x, d ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
             p[c + d] = pf_pack<BF16>(x.x, x.y);
             if (kRest) {
-              const float2 y = h2f2(p[c + d]);
-              rest[kRest ? c + d : 0] = pf_pack<false>(x.x - y.x, x.y - y.y);
+              const uint32_t u = p[c + d];
+              const float2 y = BF16 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)) : h2f2(u);
+              rest[kRest ? c + d : 0] = pf_pack<BF16>(x.x - y.x, x.y - y.y);
             }
           }
         }
