@@ -236,6 +236,35 @@ def test_calls_behind_one_another_give_the_same_bits(kind, B, Hkv, Np, N):
     ops.check_status(torch.device(DEV))
 
 
+def test_offsets_beyond_32_bits():
+    """The last tokens of the last row of a cache whose codes take 3.2 GB each: written, read back and attended
+    to; and as a shared prefix seen by 24 queries per key."""
+    from topk_attn_b200 import ops
+    B, N, H = 3, 1 << 20, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.empty(B, N, H, 128, dtype=torch.int8, device=DEV).random_(-127, 128, generator=g) for _ in range(2))
+    ks, vs = (torch.rand(B, H, N, generator=g, device=DEV) * 0.01 + 0.01 for _ in range(2))
+    cache = ops.QuantizedKV(k, v, ks, vs)
+    rows = torch.randn(B, 3, H, 128, generator=g, device=DEV).half()
+    ops.kv_append_quantized(cache, rows, -rows, N - 3)
+    kb, vb = ops.kv_dequantize(cache, N - 4, 4)
+    want = O.quantize(rows.cpu(), "int8")[2]
+    assert (kb[:, 1:].cpu().double() - want).abs().max() <= want.abs().max() * 2.0 ** -11
+    assert torch.equal(kb[:, 1:], -vb[:, 1:])
+    q = torch.randn(B, 8 * H, 128, generator=g, device=DEV).half()
+    q[2, -8:, :] = rows[2, 2, -1] * 0.5        # the last head's queries look at its last token
+    out = ops.flash_decoding_quantized(q, cache, SM)
+    one = ops.QuantizedKV(k[2], v[2], ks[2], vs[2])
+    shared = ops.shared_prefix_attention(q, one, None, SM)
+    ops.check_status(torch.device(DEV))
+    kd, vd = (c[2, :, H - 1].double() * s[2, H - 1].double()[:, None] for c, s in ((k, ks), (v, vs)))
+    for b, got in ((2, out), (2, shared), (0, shared)):
+        ref = torch.softmax(q[b, -8:].double() @ kd.T * SM, -1) @ vd
+        qb = q[b:b + 1, -8:].cpu()
+        tol = O.tolerance(ref.cpu(), qb, SM, [kd[:, None].cpu()], [vd[:, None].cpu()], N, torch.float16, "int8")
+        assert ((got[b, -8:].double() - ref).abs().cpu() <= tol).all()
+
+
 def test_a_decode_loop_over_a_quantised_prefix_and_cache():
     """The operators together: a prompt is quantised once into a shared cache, then every step appends one
     token to each row's own cache and attends over both; and reading the caches back gives what the
