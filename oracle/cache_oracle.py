@@ -86,3 +86,65 @@ def tolerance(ref, q, sm_scale, ks, vs, total, dtype, kind=""):
     d = score * (130 * 2.0 ** -24 + (2.0 ** -10 if kind == "int4" else 0.0)) + 2.0 ** -22 + weight
     d += total * (2.0 ** -25 + 2.0 ** -24)
     return 2 * d * vmax + (2.0 ** -10 * vmax if kind == "int4" else 0.0) + half * ref.abs()
+
+
+#: What a kernel may add to a code while it multiplies it: int8 codes go through as code + 128, int4 ones as code + 8.
+LIFT = {"int8": 128.0, "int4": 8.0}
+
+
+def attention_terms(q, sm_scale, prefix=None, own=None, lens=None, scales=None, kind=""):
+    """What an error bound needs beside the result: (out, mass, reach), float64 on q's device.  mass = sum w |v| of each
+    element; reach [B,Hq] = sm_scale * the largest sum |q| (|k| + LIFT s) of any token, s its K scale.  ``scales``: the K
+    scales [..., N, H] (int4: the largest of a row's four) of the prefix and of the own caches, where kind has them."""
+    B, Hq, D = q.shape
+    heads = (prefix or own)[0].size(-2)
+    g = Hq // heads
+    out, mass = (torch.zeros(B, Hq, D, dtype=torch.float64, device=q.device) for _ in range(2))
+    reach = torch.zeros(B, Hq, dtype=torch.float64, device=q.device)
+    for b in range(B):
+        ks, vs, lift = [], [], []
+        for i, part in enumerate((prefix, own)):
+            if part is None:
+                continue
+            n = part[0].size(-3) if i == 0 or lens is None else max(0, min(part[0].size(1), int(lens[b])))
+            k, v = (x[:n] if i == 0 else x[b, :n] for x in part)
+            ks.append(k.double())
+            vs.append(v.double())
+            s = torch.zeros(n, heads, device=q.device) if kind not in LIFT else (scales[i][:n] if i == 0 else scales[i][b, :n]).abs() * LIFT[kind]
+            lift.append(s.double())
+        k, v, lift = torch.cat(ks), torch.cat(vs), torch.cat(lift)
+        if k.size(0) == 0:
+            continue
+        qb = q[b].double().view(heads, g, D)
+        w = torch.softmax(torch.einsum("hgd,nhd->hgn", qb, k) * sm_scale, -1)
+        out[b] = torch.einsum("hgn,nhd->hgd", w, v).reshape(Hq, D)
+        mass[b] = torch.einsum("hgn,nhd->hgd", w, v.abs()).reshape(Hq, D)
+        far = torch.einsum("hgd,nhd->hgn", qb.abs(), k.abs() + lift[..., None])
+        reach[b] = far.amax(-1).reshape(Hq) * sm_scale
+    return out, mass, reach
+
+
+def half_step(ref, dtype):
+    """Half a step of dtype at ref: what rounding alone may be off by."""
+    info = torch.finfo(dtype)
+    _, e = torch.frexp(ref.abs().clamp_min(info.tiny))
+    return torch.ldexp(torch.full_like(ref, info.eps / 2), e - 1)
+
+
+def bound(ref, mass, reach, tokens, dtype):
+    """The most that a result may be off: half a step of its type, and what its terms' roundings contribute.
+
+    A weight is held as a 16-bit value, cut off, and the 16-bit rest of it, rounded: a step of the one times half a
+    step of the other, 2^-7 2^-8 = 2^-15 (bf16) or 2^-10 2^-11 = 2^-21 (fp16).  Its score is an fp32 sum of 8 products of 16
+    dims, each at most 2^-23 of the terms' magnitude off, and a few more roundings: 2^-19 reach, which is a relative
+    error of the weight.  The hardware's exp2 adds 2^-22, the argument's rounding as much.  All of these enter the sum of
+    the values and the sum of the weights: twice.  Sums over the tokens take two steps for every 16 of them, each at
+    most 2^-23 of the magnitude; joining parts takes fewer."""
+    weight = 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -21
+    d = 2 * (weight + 2.0 ** -19 * reach[..., None] + 2.0 ** -21) + (tokens / 8 + 64) * 2.0 ** -23
+    return half_step(ref, dtype) + d * mass
+
+
+def moved(out, ref):
+    """Share of the elements that are not the correctly rounded result."""
+    return float((out != ref.to(out.dtype)).double().mean())

@@ -1,0 +1,78 @@
+"""How exact the attention over caches is: results against 64 bits, element by element, within half a step of their
+type and what the fp32 sums and the weights' two 16-bit parts leave; and long caches whose every tile counts."""
+import math
+
+import pytest
+import torch
+
+from oracle import cache_oracle as O
+from test_gpu_prefix_attention import DEV, DTYPES, KINDS, SM, device_cache, make
+
+pytestmark = pytest.mark.gpu
+
+
+def row_scales(held, kind):
+    """K scales [..., N, H] of a cache of make(), the largest of a row's for int4."""
+    if held is None or not kind:
+        return None
+    s = held[1][0][1]
+    return (s.amax(-1) if kind == "int4" else s).transpose(-2, -1)
+
+
+def terms(q, prefix, own, kind, lens=None):
+    dev = [None if p is None else tuple(x.to(DEV) for x in p[0]) for p in (prefix, own)]
+    sc = [None if p is None or not kind else row_scales(p, kind).to(DEV) for p in (prefix, own)]
+    return O.attention_terms(q.to(DEV), SM, dev[0], dev[1], lens, sc, kind)
+
+
+def attend(q, prefix, own, kind, lens=None):
+    from topk_attn_b200 import ops
+    dl = None if lens is None else lens.to(DEV)
+    out = ops.shared_prefix_attention(q.to(DEV), device_cache(prefix, kind), device_cache(own, kind), SM, dl)
+    ops.check_status(torch.device(DEV))
+    return out
+
+
+# One query tile of each kernel and two of them, own caches with whole and with odd lengths.
+SHAPES = [(3, 16, 2, 0, 200), (2, 12, 1, 0, 77), (2, 8, 4, 300, 40), (24, 8, 4, 333, 17), (90, 4, 1, 400, 9), (300, 1, 1, 257, 5)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,Hq,Hkv,Np,N", SHAPES)
+def test_the_results_own_rounding_is_what_counts(B, Hq, Hkv, Np, N, kind, dtype):
+    """An error of e steps moves a share e of the elements to another value.  The rest of a weight leaves a random
+    2^-16 (bf16) of it at most, 2^-8 of a step of the result, over a result that is a few times smaller than its terms:
+    about 1 %.  fp16: 2^-22 and the scores' fp32 sums, 2^-21 for scores of magnitude 4 and terms as many times larger: 2^-10
+    of a step, again a few times that.  Weights rounded once to the result's type move 20 to 40 % (the same inputs in
+    64 bits otherwise), fp16 weights of bf16 results an eighth of it."""
+    q, prefix, own = make(B, Hq, Hkv, Np, N, kind, dtype, 31 * B + N)
+    q = (q.float() / 2).to(dtype)
+    ref, mass, reach = terms(q, prefix, own, kind)
+    out = attend(q, prefix, own, kind)
+    far = (out.double() - ref).abs()
+    assert (far <= O.bound(ref, mass, reach, Np + N, dtype)).all()
+    assert O.moved(out, ref) <= 0.02
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B", [2, 40])
+def test_an_infinite_value_stays_one(B, dtype):
+    """A value of infinity that is attended to gives an infinity and no NaN, also for a weight of a power of two.  Weights
+    are at least 2^10 for the largest of a row, and fp16's least number is 2^-24 (2^-25 rounds to nothing): one below
+    2^-34 of the largest may be zero in the product, and zero times an infinity is a NaN."""
+    q, prefix, own = make(B, 4, 2, 200, 30, "", dtype, 8)
+    prefix[1][1][7, 0, 5] = math.inf
+    own[1][1][1, 29, 1, 3] = -math.inf
+    q[0] = 0                                   # all weights equal
+    out = attend(q, prefix, own, "").cpu()
+    finite = torch.ones(out.shape, dtype=torch.bool)
+    for rows, h, d, token, sign in ((range(B), 0, 5, 7, 1), ([1], 1, 3, 229, -1)):
+        for b in rows:
+            k = torch.cat((prefix[0][0][:, h], own[0][0][b, :, h])).double()
+            s = q[b, 2 * h:2 * h + 2].double() @ k.T * SM / math.log(2)
+            seen = s[:, token] - s.amax(-1) >= -33
+            finite[b, 2 * h:2 * h + 2, d] = False
+            got = out[b, 2 * h:2 * h + 2, d]
+            assert (got[seen] == sign * math.inf).all() and not torch.isfinite(got).any()
+    assert torch.isfinite(out[finite]).all()

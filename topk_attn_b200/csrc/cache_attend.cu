@@ -14,9 +14,10 @@
 // 16 (int4: 4) bytes of a row; V's dims come out in the order the lanes hold them.
 //
 // The running maximum moves only when a score exceeds it by 2^4 (a vote, no reduction).  Weights are
-// exp2(score - maximum + 10), at most 2^14 (2^15 with a V scale): fp32 sums do not mind, and fp16, to
-// which they are rounded for the product (bf16 for a bf16 cache), keeps its eleven bits down to 2^-24
-// of the largest.
+// exp2(score - maximum + 10), at most 2^14 (2^15 with a V scale): fp32 sums do not mind.  For the product
+// they are split into a 16-bit value and the 16-bit rest of it, which takes two MMAs: fp16 (bf16 for a bf16
+// cache) alone would add an error of the size of the result's own rounding, both parts leave 2^-21 (2^-15)
+// of a weight.
 // Bytes bound it where arithmetic does not: 512 per token and kv head in 16 bits, 264 in 8, 160 in 4.  16
 // rows behind 131072 fp16 tokens of 32 heads take 330 us (2.17 GB at 6.6 TB/s, the copy rate); 8 x 32768
 // tokens of 8 heads take 106 us in int8 (5.2 TB/s) and 95 in fp8 (5.8), where turning codes into fp16 keeps
@@ -109,6 +110,24 @@ __device__ __forceinline__ void codes_of(uint32_t w, uint32_t& first, uint32_t& 
         : "r"(w));
   }
 }
+// A pair of weights as 16-bit values and the 16-bit rests of them.  FINITE: they meet codes, which are finite;
+// both parts are rounded to nearest.  Otherwise the value is cut off a little below the weight, so that neither
+// part of a weight that counts is zero or negative: zero times an infinity of V would make a NaN of it.
+template <bool BF16, bool FINITE>
+__device__ __forceinline__ void split_pair(float lo, float hi, uint32_t& value, uint32_t& rest) {
+  constexpr float kBelow = 0.99999904632568359375f;     // 1 - 2^-20
+  float2 y;
+  if (FINITE) {
+    value = pack_pair<BF16>(lo, hi);
+  } else if (BF16) {
+    value = __byte_perm(__float_as_uint(lo * kBelow), __float_as_uint(hi * kBelow), 0x7632);
+  } else {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(value) : "f"(hi * kBelow), "f"(lo * kBelow));
+  }
+  if (BF16) y = make_float2(__uint_as_float(value << 16), __uint_as_float(value & 0xffff0000u));
+  else y = h2f2(value);
+  rest = pack_pair<BF16>(lo - y.x, hi - y.y);
+}
 // The same pairs of an int8 word as fp16 subnormals of (code + 128) 2^-24: for the scores, whose sum of q
 // times 128 goes into the accumulators beforehand.  (For the values it would not do: their long sums
 // would lose in the difference.)
@@ -144,11 +163,6 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
   constexpr int kStage = 2 * kKBytes;
   constexpr int kNS = kDense ? 1 : cache_row_scales(FMT);
   constexpr int kScaleFloats = attend_scale_floats(FMT);
-  // fp16 results of 8-bit caches: the weights go through the product as an fp16 value and the fp16 rest of
-  // it.  Rounded once they would add as much error again as the result's own rounding (2.0e-4 of its norm
-  // each, 3.1e-4 together over 32768 tokens).  The eight more MMAs cost up to 9 % of the time (int8, 8 x
-  // 32768 tokens on 384 CTAs: 113 us with them, 104 without).
-  constexpr bool kRest = !kDense && !BF16 && kNS == 1;
   constexpr int QT = 8 * NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
@@ -598,7 +612,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
             }
         }
         // ---- weights, scaled by V's scales, as B fragments (tokens along k)
-        uint32_t pb[NQ][kNS][2], pr[kRest ? NQ : 1][2];
+        uint32_t pb[NQ][kNS][2], pr[NQ][kNS][2];
         const float down = kDense ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(c_ref));
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
@@ -610,14 +624,13 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 #pragma unroll
           for (int j = 0; j < kNS; ++j) {
             const float f0 = kDense ? 1.f : vs[0][j] * down, f1 = kDense ? 1.f : vs[1][j] * down;
-            const uint32_t a = pack_pair<kPBf16>(p[0] * f0, p[1] * f0), c = pack_pair<kPBf16>(p[2] * f1, p[3] * f1);
+            uint32_t a, ar, c, cr;
+            split_pair<kPBf16, !kDense>(p[0] * f0, p[1] * f0, a, ar);
+            split_pair<kPBf16, !kDense>(p[2] * f1, p[3] * f1, c, cr);
             pb[nq][j][0] = movmatrix_trans(a);
             pb[nq][j][1] = movmatrix_trans(c);
-            if (kRest) {
-              const float2 fa = h2f2(a), fc = h2f2(c);
-              pr[kRest ? nq : 0][0] = movmatrix_trans(pack_pair<false>(p[0] * f0 - fa.x, p[1] * f0 - fa.y));
-              pr[kRest ? nq : 0][1] = movmatrix_trans(pack_pair<false>(p[2] * f1 - fc.x, p[3] * f1 - fc.y));
-            }
+            pr[nq][j][0] = movmatrix_trans(ar);
+            pr[nq][j][1] = movmatrix_trans(cr);
           }
         }
         // ---- O^T += V^T P^T
@@ -637,7 +650,10 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
               a[0] &= k0; a[1] &= k0; a[2] &= k1; a[3] &= k1;
             }
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) mma_any<kPBf16>(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
+            for (int nq = 0; nq < NQ; ++nq) {
+              mma_any<kPBf16>(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
+              mma_any<kPBf16>(o[nq][mt], a, pr[nq][0][0], pr[nq][0][1]);
+            }
           }
         } else if (FMT == kCacheInt4) {
           // lane g: dims 32 j + 4 g .. + 3 of group j, two bytes of a token
@@ -656,8 +672,10 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
               const uint32_t a[4] = {nibbles_of(w[0], 2 * i), nibbles_of(w[0], 2 * i + 1), nibbles_of(w[1], 2 * i),
                                      nibbles_of(w[1], 2 * i + 1)};
 #pragma unroll
-              for (int nq = 0; nq < NQ; ++nq)
+              for (int nq = 0; nq < NQ; ++nq) {
                 mma_16816(o[nq][2 * j + i], a, pb[nq][j < kNS ? j : 0][0], pb[nq][j < kNS ? j : 0][1]);
+                mma_16816(o[nq][2 * j + i], a, pr[nq][j < kNS ? j : 0][0], pr[nq][j < kNS ? j : 0][1]);
+              }
             }
           }
         } else {
@@ -684,7 +702,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
               mma_16816(o[nq][mt], a, pb[nq][0][0], pb[nq][0][1]);
-              if (kRest) mma_16816(o[nq][mt], a, pr[kRest ? nq : 0][0], pr[kRest ? nq : 0][1]);
+              mma_16816(o[nq][mt], a, pr[nq][0][0], pr[nq][0][1]);
             }
           }
         }

@@ -14,7 +14,9 @@
 //   warps 4-11  softmax: a thread owns one query (one TMEM lane), so maximum and sum need no exchange;
 //               P goes back into S's columns as the A operand of the second product
 // The maximum moves only when a score exceeds it by 2^4, and only then O is rescaled in TMEM; no wait
-// is needed for that: S(k) is committed after O's product k-1.  Weights are rounded to the type of V.
+// is needed for that: S(k) is committed after O's product k-1.  Weights go through the product as a value of V's
+// type and, in the other half of S's columns, the rest of it in the same type, so that the result's own rounding
+// is the only one that counts.
 //
 // 256 batch rows x 32 heads behind 32768 bf16 tokens of 8 kv heads: 134-150 us for this kernel, 0.92-1.03
 // PFLOP/s, with the tensor pipe at 49 %: a pair of steps takes about 3050 cycles, 2048 of them products, and
@@ -168,6 +170,22 @@ __device__ __forceinline__ uint32_t pf_pack(float lo, float hi) {
   return r;
 }
 
+// A pair of weights as 16-bit values and the 16-bit rests of them.  FINITE: they meet codes, which are finite;
+// both parts are rounded to nearest.  Otherwise the value is cut off a little below the weight, so that neither
+// part of a weight that counts is zero or negative: zero times an infinity of V would make a NaN of it.
+template <bool BF16, bool FINITE>
+__device__ __forceinline__ void pf_split(float2 x, uint32_t& value, uint32_t& rest) {
+  if (FINITE) {
+    value = pf_pack<BF16>(x.x, x.y);
+  } else {
+    const float2 y = mul2(x, make_float2(0.99999904632568359375f, 0.99999904632568359375f));   // 1 - 2^-20
+    if (BF16) value = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
+    else asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(value) : "f"(y.y), "f"(y.x));
+  }
+  const float2 z = BF16 ? make_float2(__uint_as_float(value << 16), __uint_as_float(value & 0xffff0000u)) : h2f2(value);
+  rest = pf_pack<BF16>(x.x - z.x, x.y - z.y);
+}
+
 // Sixteen codes as eight pairs of fp16 or bf16.
 template <int FMT, bool BF16>
 __device__ __forceinline__ void pf_codes(const uint4& u, uint32_t (&r)[8]) {
@@ -202,9 +220,6 @@ template <int FMT, bool BF16>
 __global__ void __launch_bounds__(pf_threads(FMT >= kCacheInt8), 1)
 prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
   constexpr bool kCodes = FMT >= kCacheInt8;
-  // 8-bit caches: the weights go through the product as an fp16 (bf16) value and, in the other half of S's
-  // columns, the rest of it in the same type, so that the result's own rounding is the only one that counts
-  constexpr bool kRest = kCodes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -360,7 +375,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
           for (int c = 0; c < kPrefixEarly / 16; ++c) {
             tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, c > 0 ? 1u : add);
-            if (kRest) tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+            tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
           }
         }
         __syncwarp();
@@ -371,7 +386,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
           for (int c = kPrefixEarly / 16; c < 8; ++c) {
             tc_mma_ts(tm_o, tm_s + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
-            if (kRest) tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
+            tc_mma_ts(tm_o, tm_s + 64 + 8 * c, b + (uint64_t)(c * 2048 >> 4), kIdO, 1u);
           }
           tc_commit(&ctrl->empty[s]);
           if (!more) tc_commit(&ctrl->o_full[st]);
@@ -559,7 +574,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int part = 0; part < 4; ++part) {
-        uint32_t p[16], rest[kRest ? 16 : 1];
+        uint32_t p[16], rest[16];
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
           const int e = 32 * part + 2 * c;
@@ -573,16 +588,11 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
             x.y = fast_exp2(x.y);
             sum[d] = add2(sum[d], x);
             if (kCodes) x = mul2(x, d ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
-            p[c + d] = pf_pack<BF16>(x.x, x.y);
-            if (kRest) {
-              const uint32_t u = p[c + d];
-              const float2 y = BF16 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)) : h2f2(u);
-              rest[kRest ? c + d : 0] = pf_pack<BF16>(x.x - y.x, x.y - y.y);
-            }
+            pf_split<BF16, kCodes>(x, p[c + d], rest[c + d]);
           }
         }
         tc_st16(tms + 16 * part, p);
-        if (kRest) tc_st16(tms + 64 + 16 * part, rest);
+        tc_st16(tms + 64 + 16 * part, rest);
         if (part == kPrefixYield) mbar_arrive(&ctrl->turn[st ^ 1]);
         if (part == kPrefixEarly / 32 - 1 || part == 3) {
           tc_wait_st();
