@@ -408,7 +408,8 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     const int t = tid - 384;
     const long long at = (long long)h * P.scale_hstride + (long long)tile0 * kPrefixTile + t;
     const int left = P.n_tokens - tile0 * kPrefixTile - t;       // tokens from mine on
-    float ks = left > 0 ? __ldg(P.k_scale + at) : 0.f, vs = left > 0 ? __ldg(P.v_scale + at) : 0.f;
+    auto scale = [](const float* p) { return __uint_as_float(ld32(p)); };
+    float ks = left > 0 ? scale(P.k_scale + at) : 0.f, vs = left > 0 ? scale(P.v_scale + at) : 0.f;
     // V of tile j and K of tile j + stride together: one round of waits, one fence
     int n = 0;                                       // code tiles so far
     for (int j = -stride; j < tiles; ++j) {
@@ -460,8 +461,8 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         if (lane == 0) scales->top[sj][t >> 5] = top;
         mbar_arrive(&ctrl->scales_full[sj]);
         const bool next = left > (jk + 1) * kPrefixTile;
-        ks = next ? __ldg(P.k_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
-        vs = next ? __ldg(P.v_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
+        ks = next ? scale(P.k_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
+        vs = next ? scale(P.v_scale + at + (long long)(jk + 1) * kPrefixTile) : 0.f;
       }
     }
   } else {
@@ -481,7 +482,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         u[i] = make_uint4(0u, 0u, 0u, 0u);
         if (i < n && first + 16 * i < P.queries) {
           const long long row = (long long)qb * P.hq + h * P.group + qg;
-          u[i] = ldg128_nc(static_cast<const unsigned char*>(P.q) + row * kRowBytes + 16 * c);
+          u[i] = ld128(static_cast<const unsigned char*>(P.q) + row * kRowBytes + 16 * c);
         }
         qb += step_b;
         qg += step_g;

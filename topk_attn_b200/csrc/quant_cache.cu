@@ -114,8 +114,8 @@ kv_quantize_kernel(const __grid_constant__ QuantParams P) {
       u[i][0] = u[i][1] = make_uint4(0u, 0u, 0u, 0u);
       if (r0 + i * kSlots + slot < rows) {
         const unsigned char* at = src + load.t * rt + load.h * rh;
-        u[i][0] = ldg128_nc(at);
-        u[i][1] = ldg128_nc(at + 128);
+        u[i][0] = ld128(at);
+        u[i][1] = ld128(at + 128);
       }
       load.step(dt, dh, heads);
     }
@@ -264,7 +264,7 @@ kv_dequantize_kernel(const __grid_constant__ QuantParams P) {
   const int dk = kQuantThreads % run, ds = kQuantThreads / run;
   for (int i = threadIdx.x, h = i / run, k = i % run; i < rows * kScales; i += kQuantThreads) {
     const int t = k / kScales;
-    sm_scale[i] = t >= lo && t < hi ? scales[h * P.cache.shstride + k] : 0.f;
+    sm_scale[i] = t >= lo && t < hi ? __uint_as_float(ld32(scales + h * P.cache.shstride + k)) : 0.f;
     h += ds;
     k += dk;
     if (k >= run) {
@@ -287,8 +287,8 @@ kv_dequantize_kernel(const __grid_constant__ QuantParams P) {
         const unsigned char* at = codes + load.t * P.cache.tstride + load.h * P.cache.hstride;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (FMT == kCacheInt4) u[i][c].x = __ldg(reinterpret_cast<const uint32_t*>(at + 4 * lane8 + 32 * c));
-          else u[i][c] = __ldg(reinterpret_cast<const uint2*>(at + 8 * lane8 + 64 * c));
+          if (FMT == kCacheInt4) u[i][c].x = ld32(at + 4 * lane8 + 32 * c);
+          else u[i][c] = ld64(at + 8 * lane8 + 64 * c);
         }
       }
       load.step(dt, dh, heads);

@@ -29,6 +29,25 @@ struct CacheView {
   long long sbstride, shstride;
 };
 
+// Loads of what an earlier kernel may have written while this one, launched early, was already there: after
+// griddepcontrol.wait, and not through the read-only path, which is for data that nobody writes as long as the
+// kernel lives.  Volatile, so that they stay behind the wait.
+__device__ __forceinline__ uint4 ld128(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ld64(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld32(const void* p) {
+  uint32_t r;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+
 constexpr int kQuantMaxHeads = 1024;
 
 struct QuantParams {
