@@ -76,3 +76,31 @@ def test_an_infinite_value_stays_one(B, dtype):
             got = out[b, 2 * h:2 * h + 2, d]
             assert (got[seen] == sign * math.inf).all() and not torch.isfinite(got).any()
     assert torch.isfinite(out[finite]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("B,Np", [(24, 61440), (150, 30720)])
+def test_a_long_run_of_zero_values(B, Np, kind, dtype):
+    """Values that are all zero (their scale is zero too), with scores a little below what moves the running maximum (4
+    binary units, 2.77 natural ones): the sum of the weights stays finite, and what follows has its share."""
+    from topk_attn_b200 import ops
+    H = 149                               # so many heads that the tokens are not split
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q = torch.ones(B, H, 128, device=DEV, dtype=dtype)
+    prefix = ops.quantized_kv_cache(Np, H, kind, device=DEV)
+    v = torch.randn(256, H, 128, generator=g, device=DEV).to(dtype)
+    zero = torch.zeros(1, 1, 128, device=DEV, dtype=dtype)
+    for at, n, score, value in ((256, Np - 512, 2.7, zero.expand(Np - 512, H, 128)), (Np - 256, 256, 6.0, v)):
+        ops.kv_append_quantized(prefix, (zero + score / (128 * SM)).expand(n, H, 128), value, at)
+    out = ops.shared_prefix_attention(q, prefix, None, SM)
+    ops.check_status(torch.device(DEV))
+    k = prefix.k[:, 0].double() * prefix.k_scale[0].double()[:, None]
+    w = torch.softmax(k.sum(-1) * SM, -1)[-256:]
+    val = prefix.v[-256:].double() * prefix.v_scale.t()[-256:].double()[..., None]
+    ref, mass = (torch.einsum("n,nhd->hd", w, x).expand(B, H, 128) for x in (val, val.abs()))
+    # sum |q| (|k| + 128 s): a code of a constant row is 127 (int8), so at most twice and a little more than 6
+    reach = torch.full((B, H), 13.0, dtype=torch.float64, device=DEV)
+    most = O.bound(ref, mass, reach, Np, dtype)
+    assert (ref.abs() > 4 * most).double().mean() > 0.5          # zeros would be seen
+    assert ((out.double() - ref).abs() <= most).all()

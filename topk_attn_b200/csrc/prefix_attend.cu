@@ -46,7 +46,7 @@ constexpr int kPrefixEarly = 64;                // tokens of P whose product sta
 // Quarter of P after which the other stream's turn at the exponentials begins: 145 us at the sizes above
 // against 146 with the last quarter, 167 with the second.
 constexpr int kPrefixYield = 2;
-constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f;
+constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f, kPfLeastScale = -60.f;
 
 struct PrefixScales {
   float k[kScaleTiles][kPrefixTile];    // times the score scale
@@ -545,9 +545,10 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if (kCodes) {
         // the weights are multiplied by V's scales: the reference counts their largest in, and since sums
-        // and weights share the reference, it drops out in the end
+        // and weights share the reference, it drops out in the end.  No less than 2^-60 of it: a weight is at most
+        // 2^(14 + 60) then, and 2^31 of them, of rows that are all zeros, are still a finite sum
         const float top = fmaxf(fmaxf(scales->top[sj][0], scales->top[sj][1]), fmaxf(scales->top[sj][2], scales->top[sj][3]));
-        mx += fmaxf(-100.f, (float)((int)(__float_as_uint(top) >> 23) - 126));
+        mx += fmaxf(kPfLeastScale, (float)((int)(__float_as_uint(top) >> 23) - 126));
       } else {
         mx *= P.scale_log2e;
       }
