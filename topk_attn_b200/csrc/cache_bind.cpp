@@ -22,7 +22,7 @@ using OptTensor = c10::optional<Tensor>;
 
 [[noreturn]] void refuse(const std::string& why) { throw py::value_error(why); }
 
-// The zeroed status block of a device, shared by its streams: kernels only set bits in it.
+// The status block of a device, shared by its streams and graphs: kernels only set bits in it.
 std::mutex g_mu;
 std::map<int, Tensor> g_status;
 
@@ -31,17 +31,26 @@ bool capturing(cudaStream_t stream) {
   return cudaStreamIsCapturing(stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
 }
 
-// A graph captured before any eager call on the device gets a block of its own, which nobody reads.
-Tensor status_for(const torch::Device& dev, cudaStream_t stream) {
+// The block outlives every graph whose kernels write it, also one captured before any eager call on the device:
+// it is no part of the capture, so it comes from cudaMalloc in a thread whose capture mode lets that pass, and is
+// zeroed on a stream of its own.
+Tensor status_for(const torch::Device& dev) {
   std::lock_guard<std::mutex> g(g_mu);
   auto it = g_status.find(dev.index());
   if (it != g_status.end()) return it->second;
-  auto t = torch::zeros({256}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
-  if (!capturing(stream)) {
-    cudaStreamSynchronize(stream);   // other streams use it from now on
-    g_status[dev.index()] = t;
-  }
-  return t;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  void* p = nullptr;
+  cudaStream_t own = nullptr;
+  cudaError_t e = cudaMalloc(&p, 256);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, own);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+  if (own) cudaStreamDestroy(own);
+  if (e != cudaSuccess && p) cudaFree(p);
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  C10_CUDA_CHECK(e);
+  return g_status[dev.index()] = torch::from_blob(p, {256}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
 }
 
 // Scratch for one call: the stream's buffer, grown on demand (an outgrown one may still be in use by
@@ -184,7 +193,7 @@ int kv_rows(bool back, const Tensor& ck, const Tensor& cv, const Tensor& cks, co
   if (counts) p.counts = int32_vector(*counts, c.caches, dev, "counts");
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   p.stream = stream;
-  const Tensor status = status_for(dev, stream);
+  const Tensor status = status_for(dev);
   p.status = status.data_ptr();
   return back ? ra_kv_dequantize(&p) : ra_kv_append_quantized(&p);
 }
@@ -253,7 +262,7 @@ std::pair<int, Tensor> cache_attention(const Tensor& q, const OptTensor& pk, con
   p.stream = stream;
   const size_t need = ra_cache_attention_workspace_bytes(p.batch, p.num_q_heads, p.num_kv_heads, p.prefix.num_tokens,
                                                          p.cache.num_tokens);
-  const Tensor ws = scratch_for(std::max<size_t>(need, 256), dev, stream), status = status_for(dev, stream);
+  const Tensor ws = scratch_for(std::max<size_t>(need, 256), dev, stream), status = status_for(dev);
   p.workspace = ws.data_ptr();
   p.workspace_bytes = (size_t)ws.numel();
   p.status = status.data_ptr();
