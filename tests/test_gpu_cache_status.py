@@ -52,3 +52,48 @@ for g, bad in zip(graphs, (at, at, lens)):
     ops.check_status()
 print("all reported")
 """, "all reported")
+
+
+def test_scratch_of_a_growing_batch_is_bounded():
+    """A batch that grows row by row keeps one buffer of at most twice what the largest call needs."""
+    in_a_new_process("""
+import torch
+from topk_attn_b200 import capi, ops
+k, v = (torch.randn(160, 100, 8, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+q = torch.randn(160, 32, 128, device="cuda", dtype=torch.bfloat16)
+out = torch.empty_like(q)
+for b in range(1, 161):
+    ops.shared_prefix_attention(q[:b], None, (k[:b], v[:b]), 0.1, out=out[:b])
+    if b == 1:
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+torch.cuda.synchronize()
+need = max(capi.lib().ra_cache_attention_workspace_bytes(b, 32, 8, 0, 100) for b in range(1, 161))
+grown = torch.cuda.memory_allocated() - start
+assert grown <= 2 * need + (1 << 20), (grown, need)
+for i in (0, 80, 159):
+    alone = ops.shared_prefix_attention(q[i:i + 1], None, (k[i:i + 1], v[i:i + 1]), 0.1)
+    assert (out[i].double() - alone[0].double()).abs().max() <= 2.0 ** -7 * alone.double().abs().max()
+print("bounded")
+""", "bounded")
+
+
+def test_scratch_that_is_replaced_while_launches_use_it():
+    """Calls that need ever more scratch behind one another without a pause, on two streams, with other tensors taken
+    and given back between them, give what each gives alone."""
+    from topk_attn_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(3)
+    pk, pv = (torch.randn(3000, 4, 128, generator=g, device=DEV).half() for _ in range(2))
+    q = torch.randn(300, 16, 128, generator=g, device=DEV).half()
+    sizes = [1, 2, 5, 9, 17, 40, 70, 129, 200, 300]
+    want = [ops.shared_prefix_attention(q[:b].clone(), (pk, pv), None, 0.1) for b in reversed(sizes)][::-1]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        stream = torch.cuda.Stream()          # with a small buffer to begin with, whatever came before
+        got = []
+        with torch.cuda.stream(stream):
+            for b in sizes:
+                got.append(ops.shared_prefix_attention(q[:b], (pk, pv), None, 0.1))
+                torch.empty(1 << 21, dtype=torch.uint8, device=DEV).fill_(255)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))

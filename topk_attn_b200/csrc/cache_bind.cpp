@@ -53,19 +53,19 @@ Tensor status_for(const torch::Device& dev) {
   return g_status[dev.index()] = torch::from_blob(p, {256}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
 }
 
-// Scratch for one call: the stream's buffer, grown on demand (an outgrown one may still be in use by
-// launches in flight and is kept), or memory of the call's own inside a capture, because captured graphs
-// may be replayed at the same time, on any streams.
+// Scratch for one call: the stream's buffer, or memory of the call's own inside a capture, because captured graphs
+// may be replayed at the same time, on any streams.  The buffer grows to twice its size at least, and an outgrown
+// one goes back to the stream's pool, whose next user on the stream runs behind the launches that still use it.
 Tensor scratch_for(size_t bytes, const torch::Device& dev, cudaStream_t stream) {
   static std::map<std::pair<int, cudaStream_t>, Tensor> cache;
-  static std::vector<Tensor> retired;
   const auto opt = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
   if (capturing(stream)) return torch::empty({(int64_t)bytes}, opt);
   std::lock_guard<std::mutex> g(g_mu);
   Tensor& t = cache[std::make_pair((int)dev.index(), stream)];
-  if (!t.defined() || (size_t)t.numel() < bytes) {
-    if (t.defined()) retired.push_back(t);
-    t = torch::empty({(int64_t)std::max<size_t>(bytes, 1 << 20)}, opt);
+  const size_t had = t.defined() ? (size_t)t.numel() : 0;
+  if (had < bytes || !t.defined()) {
+    t = Tensor();
+    t = torch::empty({(int64_t)std::max<size_t>({bytes, 2 * had, 1 << 20})}, opt);
   }
   return t;
 }
