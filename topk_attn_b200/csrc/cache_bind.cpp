@@ -130,7 +130,6 @@ Cache cache_of(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptT
   r.c.token_stride = s.t;
   r.c.head_stride = s.h;
   if (quantized) {
-    if (!vs.has_value()) refuse("a quantised cache needs both scales");
     const int64_t w = int4 ? 4 : 1, d0 = per_row ? 1 : 0;
     int64_t hs[2], bs[2];
     for (int i = 0; i < 2; ++i) {
@@ -218,6 +217,8 @@ std::pair<int, Tensor> cache_attention(const Tensor& q, const OptTensor& pk, con
                                        const OptTensor& pvs, const OptTensor& k, const OptTensor& v,
                                        const OptTensor& ks, const OptTensor& vs, const OptTensor& seq_lens,
                                        double sm_scale, const OptTensor& out_given) {
+  if (pk.has_value() != pv.has_value() || k.has_value() != v.has_value()) refuse("a cache needs both k and v");
+  if (pks.has_value() != pvs.has_value() || ks.has_value() != vs.has_value()) refuse("a quantised cache needs both scales");
   if (!q.is_cuda()) refuse("tensors must be CUDA tensors");
   if (q.dim() != 3 || q.size(2) != 128 || !q.is_contiguous())
     refuse("q must be a contiguous fp16 or bf16 tensor [B,Hq,128]");
