@@ -332,6 +332,7 @@ typedef struct ra_cache_attention_params {
   void* stream;
 } ra_cache_attention_params;
 
+/* 0 for sizes that ra_cache_attention refuses. */
 size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                           int32_t prefix_tokens, int32_t cache_tokens);
 int ra_cache_attention(const ra_cache_attention_params* p);

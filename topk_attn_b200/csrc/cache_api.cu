@@ -21,6 +21,7 @@ int invalid(const char* why) { return host_fail(RA_ERR_INVALID_ARGUMENT, why); }
 int unsupported(const char* why) { return host_fail(RA_ERR_UNSUPPORTED, why); }
 
 constexpr int kMaxTokens = INT32_MAX - 4095;   // tiles are counted in 32 bits, rounding up
+constexpr int kMaxQueryRows = 1 << 24;
 
 bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
@@ -73,6 +74,7 @@ int check_rows(const ra_kv_rows_params* p, QuantParams& q) {
   if (p->caches < 1 || p->num_kv_heads < 1 || p->num_rows < 0) return invalid("sizes must be positive");
   if (p->caches > 65535 || p->num_kv_heads > kQuantMaxHeads)
     return unsupported("more than 65535 caches or 1024 kv heads");
+  if (p->num_rows > kMaxTokens) return unsupported("more than 2^31 - 4096 rows for a cache");
   if (p->cache.num_tokens < 1) return invalid("the cache has no tokens");
   if (p->cache.format < RA_CACHE_INT8) return invalid("the cache must be int8, fp8 or int4");
   if (p->row_type != RA_TYPE_FP16 && p->row_type != RA_TYPE_BF16) return invalid("rows must be fp16 or bf16");
@@ -230,6 +232,10 @@ int ra_kv_dequantize(const ra_kv_rows_params* p) {
 size_t ra_cache_attention_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                           int32_t prefix_tokens, int32_t cache_tokens) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || prefix_tokens < 0 || cache_tokens < 0) return 0;
+  // what ra_cache_attention refuses; the plans count rows and tiles in 32 bits
+  if (num_q_heads % num_kv_heads || (long long)batch * num_q_heads > kMaxQueryRows || prefix_tokens > kMaxTokens ||
+      cache_tokens > kMaxTokens)
+    return 0;
   // room for either kind of cache
   const int sms = host_sm_count();
   size_t need = 0;
@@ -252,7 +258,7 @@ int ra_cache_attention(const ra_cache_attention_params* p) {
   if (p->prefix.num_tokens < 0 || p->cache.num_tokens < 0) return invalid("sizes must not be negative");
   if (has[0] && has[1] && p->prefix.format != p->cache.format)
     return invalid("prefix and cache must have one format");
-  if ((long long)p->batch * p->num_q_heads > (1 << 24)) return unsupported("more than 2^24 query rows");
+  if ((long long)p->batch * p->num_q_heads > kMaxQueryRows) return unsupported("more than 2^24 query rows");
   CacheView view[2];
   for (int i = 0; i < 2; ++i) {
     const ra_kv_cache& kv = i ? p->cache : p->prefix;
