@@ -296,7 +296,8 @@ typedef struct ra_kv_rows_params {
   const int32_t* positions;      /* optional device int32 [caches]: first token of each cache */
   int32_t position;              /* first token of every cache when positions is NULL */
   const int32_t* counts;         /* append only, optional device int32 [caches]: only the first
-                                    counts[c] rows are written (a padded batch) */
+                                    counts[c] rows are written (a padded batch); clamped to
+                                    [0, num_rows] without a report */
   void* status;                  /* status block, 256 bytes, zeroed once */
   void* stream;
 } ra_kv_rows_params;

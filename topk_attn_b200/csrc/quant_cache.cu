@@ -93,7 +93,7 @@ kv_quantize_kernel(const __grid_constant__ QuantParams P) {
   const int lane8 = threadIdx.x & 7, which = blockIdx.y, b = blockIdx.z;
   const int t0 = blockIdx.x * P.tile;
   int n = min(P.tile, P.n_rows - t0);
-  if (P.counts) n = min(n, P.counts[b] - t0);
+  if (P.counts) n = min(n, max(P.counts[b], 0) - t0);
   const long long first = (long long)first_token(P, b) + t0;   // token of row t0
   if (n > 0 && (first < 0 || first + n > P.cache.n_tokens) && threadIdx.x == 0) atomicOr(P.status, kStatusBadToken);
   if (n <= 0 || first >= P.cache.n_tokens || first + n <= 0) return;

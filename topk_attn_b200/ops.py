@@ -343,7 +343,8 @@ def kv_append_quantized(cache: QuantizedKV, new_k: Tensor, new_v: Tensor, positi
     do) and store them as the tokens position .. position+T-1 of each cache.
 
     ``position`` is one int for all caches or an int32 tensor [B] ([1] for a shared cache) on the
-    device; ``counts`` int32 [B] says how many of the T rows of each are written (a padded batch).
+    device; ``counts`` int32 [B] says how many of the T rows of each are written (a padded batch; none
+    below zero, all from T on, neither is reported).
     Rows that a device-side position puts outside the cache are left out and reported by
     ``check_status``."""
     at, pos = (position, 0) if isinstance(position, Tensor) else (None, int(position))
