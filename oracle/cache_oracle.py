@@ -75,9 +75,12 @@ def tolerance(ref, q, sm_scale, ks, vs, total, dtype, kind=""):
     fp32 sums of 128 exact products: 2^-24 * 130 of sum |q||k| in every score, and a score's error
     is a relative error of its weight; exp2 in hardware 2^-22; weights rounded for the matrix
     product, half a step relative (plus 2^-25 absolute for each token where fp16 weights turn
-    subnormal); int4 values dequantised in fp16 with a rounded ratio, two half steps of fp16 in the
-    scores and the values; fp32 sums over the tokens 2^-24 each; the output's own half step.
-    A relative weight error d moves the output by at most 2 d max |v|."""
+    subnormal); for int4 two half steps of fp16 in the scores and the values, which a kernel that
+    dequantised them in fp16 would need; fp32 sums over the tokens 2^-24 each; the output's own half step.
+    A relative weight error d moves the output by at most 2 d max |v|.
+
+    A coarse bound, wider than the answer itself for int4 and for long contexts: ``bound`` is the one that tells a
+    wrong result from a right one."""
     half = torch.finfo(dtype).eps / 2
     kmax = torch.stack([k.abs().double().flatten(0, -2).amax(0) for k in ks]).amax(0)
     vmax = max(float(v.abs().max()) for v in vs)
@@ -148,3 +151,17 @@ def bound(ref, mass, reach, tokens, dtype):
 def moved(out, ref):
     """Share of the elements that are not the correctly rounded result."""
     return float((out != ref.to(out.dtype)).double().mean())
+
+
+def planted(queries, tokens, dtype, gen):
+    """Queries [R,128] and rows k, v [N,1,128] of which every tile of 64 tokens counts: one key of each points along a query
+    (the tiles take the queries in turn) with a score of 9, the others' scores are near 0."""
+    dev = gen.device
+    q = torch.randn(queries, 128, generator=gen, device=dev).to(dtype)
+    k = torch.randn(tokens, 128, generator=gen, device=dev) * 0.05
+    v = torch.randn(tokens, 128, generator=gen, device=dev)
+    tiles = torch.arange(0, tokens, 64, device=dev)
+    at = tiles + (torch.rand(tiles.numel(), generator=gen, device=dev) * (tokens - tiles).clamp(max=64)).long()
+    to = q.float()[torch.arange(tiles.numel(), device=dev) % queries]
+    k[at] = to * (9.0 * math.sqrt(128) / to.square().sum(-1, keepdim=True))
+    return q, k.to(dtype)[:, None], v.to(dtype)[:, None]
