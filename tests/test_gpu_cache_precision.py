@@ -104,3 +104,39 @@ def test_a_long_run_of_zero_values(B, Np, kind, dtype):
     most = O.bound(ref, mass, reach, Np, dtype)
     assert (ref.abs() > 4 * most).double().mean() > 0.5          # zeros would be seen
     assert ((out.double() - ref).abs() <= most).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B", [1, 20, 150])
+def test_scores_that_fp32_holds_coarsely(B, kind, dtype):
+    """Scores up to 2^36 binary units, each batch row with another magnitude: the largest one takes all of the weight, and
+    two that are the same share it.  The others are a tenth below: 2^17 units at least."""
+    from topk_attn_b200 import ops
+    H, Np = 2, 300
+    g = torch.Generator(device=DEV).manual_seed(B)
+    sign = torch.where(torch.rand(H, 128, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    c = torch.rand(Np, H, 1, generator=g, device=DEV) * 0.8 + 0.1
+    c[70, 0] = c[280, 1] = c[130, 1] = 1.0
+    v = torch.randn(Np, H, 128, generator=g, device=DEV).to(dtype)
+    for size in (300.0, 30000.0):                       # of the keys' elements
+        k = (sign * c * size).to(dtype)
+        # q . k = 128 size |q|: log2 units of 2^20.5 .. 2^36
+        top = torch.linspace(20.5 if size < 1000 else 28.0, 28.0 if size < 1000 else 35.5, max(B, 2), device=DEV)[:B]
+        q = (sign * (torch.exp2(top)[:, None, None] * math.log(2) / (128 * size * SM))).to(dtype)
+        pair = (k, v)
+        prefix = pair
+        if kind:
+            prefix = ops.quantized_kv_cache(Np, H, kind, device=DEV)
+            ops.kv_append_quantized(prefix, *pair, 0)
+            pair = ops.kv_dequantize(prefix, dtype=torch.bfloat16)
+        out = ops.shared_prefix_attention(q, prefix, None, SM)
+        ops.check_status(torch.device(DEV))
+        val = pair[1].double()
+        want = torch.stack((val[70, 0], (val[130, 1] + val[280, 1]) / 2))
+        # half a step of the result, and of bf16 where the values were read back in it; the weights' parts and fp32 sums
+        most = O.half_step(want, dtype) + (O.half_step(val.abs().amax(0), torch.bfloat16) if kind else 0) + 2.0 ** -14 * val.abs().amax(0)
+        # 2^35.5 ln 2 / (128 30000 SM) = 98900 is no fp16 number: infinite queries have no weights
+        finite = torch.isfinite(q).all(-1).all(-1)
+        assert ((out[finite].double() - want).abs() <= most).all()
+        assert torch.isnan(out[~finite]).all() and (dtype == torch.float16 or finite.all())

@@ -45,7 +45,8 @@ struct AttendCtrl {
 };
 constexpr int kMergePitch = 68;     // floats of one query's half row in the merge buffer
 constexpr int kMergeBytes = kAttendWarps * 8 * kMergePitch * 4;
-constexpr float kLazyLog2 = 4.f, kLiftLog2 = 10.f;
+// Where fp32 holds scores no finer than 1/8, the maximum is not lifted: 10 less may be 16 less after rounding.
+constexpr float kLazyLog2 = 4.f, kLiftLog2 = 10.f, kFarLog2 = 1048576.f;
 
 __device__ __forceinline__ void attend_consumer_sync() {
   asm volatile("bar.sync 1, %0;" ::"r"(32 * kAttendWarps) : "memory");
@@ -573,7 +574,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            rise |= fmaxf(x[nq][i], x[nq][i + 2]) > m_ref[nq][i] + (kLazyLog2 + kLiftLog2);
+            rise |= fmaxf(x[nq][i], x[nq][i + 2]) - m_ref[nq][i] > kLazyLog2 + kLiftLog2;
         float c_new = c_ref;
         if (!kDense) {
           float vm = 0.f;
@@ -600,7 +601,7 @@ cache_attend_kernel(const __grid_constant__ CacheAttendParams P) {
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float m_new = fmaxf(m_ref[nq][i], mx - kLiftLog2);
+              const float m_new = fmaxf(m_ref[nq][i], fabsf(mx) < kFarLog2 ? mx - kLiftLog2 : mx);
               const float alpha = fast_exp2(m_ref[nq][i] - m_new);
               m_ref[nq][i] = m_new;
               l_run[nq][i] *= alpha;

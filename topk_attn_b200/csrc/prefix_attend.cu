@@ -46,7 +46,9 @@ constexpr int kPrefixEarly = 64;                // tokens of P whose product sta
 // Quarter of P after which the other stream's turn at the exponentials begins: 145 us at the sizes above
 // against 146 with the last quarter, 167 with the second.
 constexpr int kPrefixYield = 2;
-constexpr float kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f, kPfLeastScale = -60.f;
+// From kPfFar on fp32 holds scores no finer than 1/8: the maximum is not lifted there, since 10 less may be 16 less
+// after rounding.
+constexpr float kPfFar = 1048576.f, kPfLazy = 4.f, kPfLift = 10.f, kPfNoMax = -3e38f, kPfLeastScale = -60.f;
 
 struct PrefixScales {
   float k[kScaleTiles][kPrefixTile];    // times the score scale
@@ -121,14 +123,6 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
 }
 
 // two fp32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
-        "l"(reinterpret_cast<const uint64_t&>(c)));
-  return d;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("add.rn.f32x2 %0, %1, %2;"
@@ -502,6 +496,9 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
     // ---------------------------------------------------------------- softmax
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;    // my warp's 32 TMEM lanes
     const uint32_t tms = tmem + 128u * st + lanes, tmo = tms + 256u;
+    // the running maximum in units of S (log2 units of codes, whose scale is in K's): its difference to a score is
+    // exact where it matters, however large the two are
+    const float unit = kCodes ? 1.f : P.scale_log2e, lift = kCodes ? kPfLift : fminf(kPfLift / unit, 1e38f);
     float m_ref = kPfNoMax, l = 0.f;
     int k = 0;
     bool ok = true;
@@ -543,17 +540,16 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
         for (int d = 0; d < 4; ++d)
           mx4[d] = max3(mx4[d], __uint_as_float(s[c + d]), __uint_as_float(s[c + d + 4]));
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      const bool far = !(fabsf(mx) * unit < kPfFar);
       if (kCodes) {
         // the weights are multiplied by V's scales: the reference counts their largest in, and since sums
         // and weights share the reference, it drops out in the end.  No less than 2^-60 of it: a weight is at most
         // 2^(14 + 60) then, and 2^31 of them, of rows that are all zeros, are still a finite sum
         const float top = fmaxf(fmaxf(scales->top[sj][0], scales->top[sj][1]), fmaxf(scales->top[sj][2], scales->top[sj][3]));
-        mx += fmaxf(kPfLeastScale, (float)((int)(__float_as_uint(top) >> 23) - 126));
-      } else {
-        mx *= P.scale_log2e;
+        if (!far) mx += fmaxf(kPfLeastScale, (float)((int)(__float_as_uint(top) >> 23) - 126));
       }
-      if (__any_sync(0xffffffffu, mx > m_ref + (kPfLazy + kPfLift))) {
-        const float m_new = fmaxf(m_ref, mx - kPfLift), alpha = fast_exp2(m_ref - m_new);
+      if (__any_sync(0xffffffffu, (mx - m_ref) * unit > kPfLazy + kPfLift)) {
+        const float m_new = fmaxf(m_ref, far ? mx : mx - lift), alpha = fast_exp2((m_ref - m_new) * unit);
         m_ref = m_new;
         l *= alpha;
         if (k) {
@@ -585,7 +581,8 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
             float2 x = make_float2(__uint_as_float(s[e + 2 * d]), __uint_as_float(s[e + 2 * d + 1]));
-            x = kCodes ? add2(x, neg_m) : fma2(x, scale2, neg_m);
+            x = add2(x, neg_m);
+            if (!kCodes) x = mul2(x, scale2);
             x.x = fast_exp2(x.x);
             x.y = fast_exp2(x.y);
             sum[d] = add2(sum[d], x);
@@ -605,6 +602,7 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     // ---------------------------------------------------------------- partial
+    m_ref = fmaxf(m_ref * unit, kPfNoMax);
     const int qt = pair ? qt0 + st : qt0;
     const long long slot = ((long long)h * P.query_tiles + qt) * P.splits + split;
     const int row0 = (warp & 3) * 32;                      // my warp's rows
