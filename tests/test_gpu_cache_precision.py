@@ -34,7 +34,7 @@ def attend(q, prefix, own, kind, lens=None):
 
 
 # One query tile of each kernel and two of them, own caches with whole and with odd lengths.
-SHAPES = [(3, 16, 2, 0, 200), (2, 12, 1, 0, 77), (2, 8, 4, 300, 40), (24, 8, 4, 333, 17), (90, 4, 1, 400, 9), (300, 1, 1, 257, 5)]
+SHAPES = [(3, 16, 2, 0, 200), (2, 12, 1, 0, 77), (2, 8, 4, 300, 40), (24, 8, 4, 333, 17), (90, 4, 1, 400, 9), (300, 1, 1, 257, 5), (32, 2, 2, 300, 7), (33, 2, 2, 300, 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -80,7 +80,7 @@ def test_an_infinite_value_stays_one(B, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["int8", "fp8"])
-@pytest.mark.parametrize("B,Np", [(24, 61440), (150, 30720)])
+@pytest.mark.parametrize("B,Np", [(24, 61440), (40, 61440), (150, 30720)])
 def test_a_long_run_of_zero_values(B, Np, kind, dtype):
     """Values that are all zero (their scale is zero too), with scores a little below what moves the running maximum (4
     binary units, 2.77 natural ones): the sum of the weights stays finite, and what follows has its share."""
@@ -108,7 +108,7 @@ def test_a_long_run_of_zero_values(B, Np, kind, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("B", [1, 20, 150])
+@pytest.mark.parametrize("B", [1, 20, 50, 150])
 def test_scores_that_fp32_holds_coarsely(B, kind, dtype):
     """Scores up to 2^36 binary units, each batch row with another magnitude: the largest one takes all of the weight, and
     two that are the same share it.  The others are a tenth below: 2^17 units at least."""

@@ -157,11 +157,20 @@ int prefix_splits(int blocks, int tiles, int sms) {
   return best;
 }
 
+// Queries per key up to which a prefix goes to cache_attend, 16 of them at a time; above, to prefix_attend, 128 at
+// a time.  8 kv heads, us by the one and the other: 65536 fp16 tokens, 17 to 32 queries 90 and 57; int8 76 and 114
+// to 120, 48 queries 106 and 114, 64 queries 137 and 114; fp8 64 and 83, 48 queries 90 and 83.  8192 tokens: fp16
+// 18 and 17, int8 19 and 28, fp8 17 and 20, 64 queries 25 and 18, 29 and 23, 23 and 20.  int4 has scales along the
+// dims, which prefix_attend cannot apply to S.
+int most_narrow_queries(int format) {
+  return format == RA_CACHE_INT4 ? INT32_MAX : format <= RA_CACHE_BF16 ? 16 : 32;
+}
+
 // Where every cache is equally long and held in fp8, the grid is a multiple of the rows, so that the heads,
-// whose 128-byte rows lie side by side in memory, are walked in step: 8 x 32768 tokens of 8 heads take 95 us
-// so, with 384 CTAs, and 104 with all 444 (with 4 heads 93 and 90).  Not below 5/6 of the CTAs that fit.
-// 256-byte rows do not need it; int8 and int4, bound by their arithmetic, need the CTAs (int8: 113 against
-// 102).
+// whose 128-byte rows lie side by side in memory, are walked in step: 8 x 32768 tokens of 8 heads take 94 us
+// so, with 384 CTAs, and 107 with all 444; with 4 and 2 heads, whose rows fill less of a page, 90 either way.  Not
+// below 5/6 of the CTAs that fit.  256-byte rows do not need it; int8 and int4, bound by their arithmetic, need
+// the CTAs (8 heads, in step: int8 113 against 107, int4 113 against 99).
 int grid_in_step(long long rows, int grid, int format, bool equal) {
   if (!equal || format != RA_CACHE_FP8 || rows > grid) return grid;
   const int whole = (int)(grid / rows * rows);
@@ -176,7 +185,7 @@ SegmentPlan plan_segment(bool prefix, int format, bool equal, int batch, int hq,
   s.caches = prefix ? 1 : batch;
   s.queries = prefix ? batch * group : group;
   s.nq = s.queries <= 8 ? 1 : 2;
-  const bool wide = prefix && format != RA_CACHE_INT4 && s.queries > 16;
+  const bool wide = prefix && s.queries > most_narrow_queries(format);
   s.qt = wide ? kPrefixTile : 8 * s.nq;
   s.query_tiles = (s.queries + s.qt - 1) / s.qt;
   const long long rows = (long long)s.caches * hkv * s.query_tiles;
