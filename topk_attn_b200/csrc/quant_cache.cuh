@@ -44,7 +44,7 @@ __device__ __forceinline__ uint2 ld64(const void* p) {
 }
 __device__ __forceinline__ uint32_t ld32(const void* p) {
   uint32_t r;
-  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p));
   return r;
 }
 
