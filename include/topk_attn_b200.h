@@ -315,7 +315,8 @@ int ra_kv_dequantize(const ra_kv_rows_params* p);
  * row's own cache:
  *   out[b,h] = softmax(sm_scale * q[b,h] . [K_prefix; K_b]) [V_prefix; V_b]
  * where K_b, V_b are the first seq_lens[b] tokens of row b's cache.  Either part may be absent
- * (num_tokens 0).  The prefix is read once for all rows, not once for each.  Lengths are clamped to
+ * (num_tokens 0).  The prefix is read for the rows together, not for each: once for every 256 queries of a
+ * kv head, or for every 16 where there are up to 16 (8-bit formats: 32), and always in int4.  Lengths are clamped to
  * [0, num_tokens] (one outside sets a bit of the status block); a row with nothing to attend to
  * gives zeros.  Tokens behind a row's length are not looked at, whatever they hold. */
 typedef struct ra_cache_attention_params {

@@ -1,5 +1,4 @@
 """What a graph's kernels report, and the scratch that calls keep."""
-import math
 import os
 import subprocess
 import sys
@@ -14,7 +13,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def in_a_new_process(code, word):
     res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
-    assert word in res.stdout, res.stderr[-2000:]
+    assert word in res.stdout and res.returncode == 0, res.stderr[-2000:]
 
 
 def test_a_graph_captured_before_any_other_call_reports_what_its_replays_meet():

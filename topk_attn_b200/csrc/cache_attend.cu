@@ -17,11 +17,14 @@
 // exp2(score - maximum + 10), at most 2^14 (2^15 with a V scale): fp32 sums do not mind.  For the product
 // they are split into a 16-bit value and the 16-bit rest of it, which takes two MMAs: fp16 (bf16 for a bf16
 // cache) alone would add an error of the size of the result's own rounding, both parts leave 2^-21 (2^-15)
-// of a weight.
+// of a weight, and fp16's least number 2^-35 of the largest weight times the largest V scale.  The second MMA
+// costs fp8 and 16-bit caches up to 2 %, int8 up to 9 % (113 against 104 us for 8 x 32768 tokens on 384 CTAs), int4
+// 13 % (365 against 322 us for 1 Mi tokens).
 // Bytes bound it where arithmetic does not: 512 per token and kv head in 16 bits, 264 in 8, 160 in 4.  16
 // rows behind 131072 fp16 tokens of 32 heads take 330 us (2.17 GB at 6.6 TB/s, the copy rate); 8 x 32768
-// tokens of 8 heads take 106 us in int8 (5.2 TB/s) and 95 in fp8 (5.8), where turning codes into fp16 keeps
-// the integer pipe busy 58 % of the time; 1 Mi tokens of 8 heads take 322 us in int4 (4.2 TB/s).
+// tokens of 8 heads take 100 to 107 us in int8 (5.2 to 5.5 TB/s), where turning codes into fp16 keeps the integer
+// pipe busy 60 % of the time, and 94 in fp8 (5.9); 1 Mi tokens of 8 heads take 365 us in int4 (3.7 TB/s), with no
+// pipe above 53 % and 2.4 instructions a clock.
 // Three CTAs of 160 threads to a multiprocessor: with four (96 registers) registers spill, and what then took
 // 105 us in int8 and 411 in int4 took 111 and 525.
 #include "cache_attend.cuh"

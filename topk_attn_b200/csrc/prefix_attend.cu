@@ -18,12 +18,14 @@
 // type and, in the other half of S's columns, the rest of it in the same type, so that the result's own rounding
 // is the only one that counts.
 //
-// 256 batch rows x 32 heads behind 32768 bf16 tokens of 8 kv heads: 134-150 us for this kernel, 0.92-1.03
-// PFLOP/s, with the tensor pipe at 49 %: a pair of steps takes about 3050 cycles, 2048 of them products, and
-// what bounds it is each stream's chain of S, maximum, exponentials (about 1300 cycles for 128 x 128 on the
-// 16 results a clock of the special-function unit) and O.  Computing a share of the exponentials on the FMA
-// pipe changed nothing, handing P over in four parts instead of two made it slower (170 against 149 us).
-// With 128 queries and 16385 int8 tokens it takes about 30 us, bound by the conversion of codes.
+// 256 batch rows x 32 heads behind 32768 bf16 tokens of 8 kv heads: 185 us for this kernel, 0.74 PFLOP/s of the
+// formula's operations and half as many again for the rests, with the tensor pipe at 63 %: a pair of steps takes
+// about 4750 cycles, 3072 of them products, and what bounds it is each stream's chain of S, maximum, exponentials
+// (about 1300 cycles for 128 x 128 on the 16 results a clock of the special-function unit), rests and O.  Without
+// the rests it took 134-150 us, and then a share of the exponentials on the FMA pipe changed nothing and handing P
+// over in four parts instead of two made it slower (170 against 149 us).
+// With 128 queries and 16385 int8 tokens it takes about 35 us, with no pipe above 23 %: one query tile leaves each
+// stream one stage for K and one for V, so the conversion of codes, the products and the softmax follow one another.
 #include "prefix_attend.cuh"
 
 #include "api_host.cuh"
@@ -43,8 +45,8 @@ __host__ __device__ constexpr int pf_threads(bool codes) { return codes ? 512 : 
 __host__ __device__ constexpr int pf_soft_regs(bool codes) { return codes ? 184 : 232; }
 constexpr int kPfOtherRegs = 40, kPfConvertRegs = 104;
 constexpr int kPrefixEarly = 64;                // tokens of P whose product starts while the rest is computed
-// Quarter of P after which the other stream's turn at the exponentials begins: 145 us at the sizes above
-// against 146 with the last quarter, 167 with the second.
+// Quarter of P after which the other stream's turn at the exponentials begins.  At the sizes above a whole call takes
+// 230 to 233 us with this quarter, the one before it or the last.
 constexpr int kPrefixYield = 2;
 // From kPfFar on fp32 holds scores no finer than 1/8: the maximum is not lifted there, since 10 less may be 16 less
 // after rounding.
@@ -435,8 +437,8 @@ prefix_attend_kernel(const __grid_constant__ PrefixAttendParams P) {
           *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d)) = make_uint4(r[0], r[1], r[2], r[3]);
           *reinterpret_cast<uint4*>(dst + swz128(t, 2 * d + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
         }
-        // only now: a barrier's arrival does not wait for shared loads that nothing has used yet, and the
-        // next tile of codes, when it comes from L2, overtook them
+        // only now that the values have been used: with the arrival directly behind the loads 820 of 2000 calls on
+        // tiles in L2 gave other results, in this order none of 3000
         mbar_arrive(&ctrl->code_empty[c]);
       }
       fence_proxy_async();

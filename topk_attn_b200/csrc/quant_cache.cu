@@ -8,8 +8,9 @@
 // back as NaN throughout instead of as wrong finite values.
 //
 // Both kernels are bound by memory: 256 bytes on one side and 132 (80 for int4) on the other for each row.
-// 2 x 16384 bf16 rows of 8 heads, K and V, take 67 us into fp8 and back (406 MB moved, 6.0 TB/s).  Eight
-// lanes share a row rather than sixteen: the work on addresses and scales halves (77 us with sixteen).
+// 2 x 16384 bf16 rows of 8 heads, K and V, take 66 us into fp8 and back (406 MB moved, 6.1 TB/s), 85 into int8 or
+// int4, whose exact quotients cost more.  Eight lanes share a row rather than sixteen: the work on addresses and
+// scales halves (77 us with sixteen).
 #include "quant_cache.cuh"
 
 namespace ra {

@@ -414,9 +414,11 @@ KVCache = Union[QuantizedKV, Tuple[Tensor, Tensor]]
 def shared_prefix_attention(q: Tensor, prefix: Optional[KVCache], cache: Optional[KVCache], sm_scale: float,
                             seq_lens: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
     """Decode attention of rows whose sequences start with one common prefix: softmax over the prefix's
-    keys followed by the row's own, in one normalisation, with the prefix read once for all rows.
+    keys followed by the row's own, in one normalisation.  The prefix is read for the rows together: once for every
+    256 queries of a kv head, or for every 16 where there are up to 16 (8-bit formats: 32), and always in int4,
+    whose time so grows with the batch.
 
-    q fp16 or bf16 [B,Hq,128]; ``prefix`` (k, v) [Np,Hkv,128] of q's type or a shared QuantizedKV;
+    q fp16 or bf16 [B,Hq,128], contiguous; ``prefix`` (k, v) [Np,Hkv,128] of q's type or a shared QuantizedKV;
     ``cache`` (k, v) [B,N,Hkv,128] or a per-row QuantizedKV of the same kind; either may be None.
     ``seq_lens`` int32 [B] on the device: how many tokens of its own cache each row sees (all when
     None; 0: the prefix only).  Returns [B,Hq,128] of q's type; a row that sees nothing gets zeros."""
