@@ -80,7 +80,7 @@ def test_an_infinite_value_stays_one(B, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["int8", "fp8"])
-@pytest.mark.parametrize("B,Np", [(24, 61440), (40, 61440), (150, 30720)])
+@pytest.mark.parametrize("B,Np", [(24, 61440), (40, 61440), (150, 32768)])
 def test_a_long_run_of_zero_values(B, Np, kind, dtype):
     """Values that are all zero (their scale is zero too), with scores a little below what moves the running maximum (4
     binary units, 2.77 natural ones): the sum of the weights stays finite, and what follows has its share."""

@@ -20,7 +20,7 @@
 //
 // 256 batch rows x 32 heads behind 32768 bf16 tokens of 8 kv heads: 185 us for this kernel, 0.74 PFLOP/s of the
 // formula's operations and half as many again for the rests, with the tensor pipe at 63 %: a pair of steps takes
-// about 4750 cycles, 3072 of them products, and what bounds it is each stream's chain of S, maximum, exponentials
+// about 4750 cycles, two thirds of them products, and what bounds it is each stream's chain of S, maximum, exponentials
 // (about 1300 cycles for 128 x 128 on the 16 results a clock of the special-function unit), rests and O.  Without
 // the rests it took 134-150 us, and then a share of the exponentials on the FMA pipe changed nothing and handing P
 // over in four parts instead of two made it slower (170 against 149 us).
